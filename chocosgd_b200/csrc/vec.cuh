@@ -1,0 +1,50 @@
+// Runs of 1 - 8 consecutive elements of fp32 / bf16 / fp16 tensors, read and written with one access and
+// held as fp32 in between (each value is rounded once, when it is stored).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+// element types of the C entry points
+#define DT_F32 0
+#define DT_BF16 1
+#define DT_F16 2
+
+template <int BYTES> struct RawVec;
+template <> struct RawVec<16> { typedef uint4 type; };
+template <> struct RawVec<8> { typedef uint2 type; };
+template <> struct RawVec<4> { typedef uint32_t type; };
+template <> struct RawVec<2> { typedef uint16_t type; };
+
+// V elements of T as they lie in memory
+template <typename T, int V> struct Vec {
+  typedef typename RawVec<sizeof(T) * V>::type Raw;
+  union { Raw raw; T e[V]; };
+  __device__ __forceinline__ Vec() {}
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  __device__ __forceinline__ void clear() { raw = Raw(); }
+};
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// one element of a tensor whose type is only known at run time
+__device__ __forceinline__ float load_any(const void* p, int dt, long long i) {
+  if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dt == DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int dt, long long i, float v) {
+  if (dt == DT_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dt == DT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+static inline int dt_bytes(int dt) { return dt == DT_F32 ? 4 : 2; }

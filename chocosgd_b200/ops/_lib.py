@@ -218,3 +218,13 @@ def stream_ptr(stream=None):
 
 def ptr(t):
     return c_void_p(t.data_ptr()) if t is not None else c_void_p(0)
+
+
+def on_device(device, fn, *args):
+    """``fn(*args)`` with ``device`` as the current device (kernels and their streams are the current device's)."""
+    import torch
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
