@@ -33,8 +33,8 @@ def last_error() -> int:
     return _declare().gated_ffn_last_error()
 
 
-def _pad8(n: int) -> int:
-    return (n + 7) // 8 * 8
+def _pad16(n: int) -> int:
+    return (n + 15) // 16 * 16
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -56,7 +56,7 @@ class _Layout:
         """Room for the operand image of a matrix, or None where it is read as it is."""
         if _aligned(t):
             return None
-        return self.add(t.shape[0] * _pad8(t.shape[1]) * (6 if t.dtype == torch.float32 else 2))
+        return self.add(t.shape[0] * _pad16(t.shape[1]) * (6 if t.dtype == torch.float32 else 2))
 
 
 def _at(base, offset):
@@ -74,8 +74,8 @@ class _GatedFfnFn(torch.autograd.Function):
         lay = _Layout()
         img = [lay.image(t) for t in (x2, wi, wo)]
         planes = 3 if x.dtype == torch.float32 else 1
-        h = lay.add(planes * m * _pad8(f) * 2)
-        z = lay.add(2 * m * _pad8(f) * 4) if train else None
+        h = lay.add(planes * m * _pad16(f) * 2)
+        z = lay.add(2 * m * _pad16(f) * 4) if train else None
         buf = torch.empty(lay.size, dtype=torch.uint8, device=x.device)
         if m:
             b = buf.data_ptr()
@@ -106,7 +106,7 @@ class _GatedFfnFn(torch.autograd.Function):
             dy2 = rows_of(dy)
             lay = _Layout()
             dy_img = lay.image(dy2)
-            dz = lay.add((3 if x2.dtype == torch.float32 else 1) * 2 * m * _pad8(f) * 2)
+            dz = lay.add((3 if x2.dtype == torch.float32 else 1) * 2 * m * _pad16(f) * 2)
             scratch = torch.empty(lay.size, dtype=torch.uint8, device=x2.device)
             b, s = buf.data_ptr(), scratch.data_ptr()
             rc = lib.gated_ffn_backward(x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
