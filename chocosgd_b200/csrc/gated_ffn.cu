@@ -78,22 +78,16 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// What these barriers hand over are operand tiles (complete_tx) and accumulators (tcgen05 fences and commits), no plain
+// memory: the default scope serves.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
-    if (ok) return true;
-    if (i > 1024) __nanosleep(64);
-  }
-  return false;
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // CG = 2: the bytes are counted on a barrier of either CTA of the pair (`bar`: a cluster address)
@@ -346,6 +340,16 @@ template <int BN, int S, int CG> struct FfnSmem {
   static constexpr int BYTES = STAGES * STAGE + 256 + 1024;
 };
 
+// Tile order: groups of FF_GROUP row tiles, rows fastest within a group, so that the tiles worked on at one time form a
+// block that is about as high as wide and share both operands' panels in L2.
+#define FF_GROUP 8
+__device__ __forceinline__ void ff_tile(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int per_group = FF_GROUP * tiles_n, group = tile / per_group, r = tile - group * per_group;
+  const int rows = min(FF_GROUP, tiles_m - group * FF_GROUP);
+  tn = r / rows;
+  tm = group * FF_GROUP + (r - tn * rows);
+}
+
 template <int BN, int S, int KIND, int CG>
 __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_constant__ FfnGemm g) {
   typedef FfnSmem<BN, S, CG> L;
@@ -390,101 +394,113 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
   pdl_wait();
   pdl_trigger();
 
-  if (warp == FF_EPI && lane == 0) {
+  // The TMA and the MMA warp run their loops as whole warps and elect a lane for the instructions alone: addresses and
+  // descriptors then stay in uniform registers.
+  if (warp == FF_EPI) {
     // ---------------- TMA producer ----------------
-    uint32_t it = 0;
+    uint32_t it = 0, s = 0, phase = 1;      // stage and the parity of its `empty` barrier (the first round passes at once)
     bool ok = true;
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step) {
-      const int tm = tile % (tiles_m * g.m_parts), n0 = (tile / (tiles_m * g.m_parts)) * BN_OUT;
-      const int m_part = tm / tiles_m, m0 = (tm % tiles_m) * TM + (int)rank * FF_BM;
-      for (int i = 0; i < n_kb; ++i, ++it) {
-        const uint32_t s = it % L::STAGES;
-        if (it >= L::STAGES && !mbar_wait_cluster(empty + s, ((it / L::STAGES) - 1) & 1)) ok = false;
-        if (*abort_flag) ok = false;
-        if (!ok) { *abort_flag = 1; break; }
-        const int seg = i / g.k_blocks, k0 = (i - seg * g.k_blocks) * FF_BK;
-        if (rank == 0) mbar_expect_tx(full + s, CG * L::STAGE);
-        const uint32_t bar = CG == 2 ? map_rank(full + s, 0) : smem_u32(full + s);
-        uint8_t* stage = smem + s * L::STAGE;
+      int tm, tn;
+      ff_tile(tile, tiles_m * g.m_parts, tiles_n, tm, tn);
+      const int n0 = tn * BN_OUT, m_part = tm / tiles_m, m0 = (tm % tiles_m) * TM + (int)rank * FF_BM;
+      for (int seg = 0; seg < g.segments && ok; ++seg) {
+        const int part_a = g.m_parts > 1 ? m_part : (g.a_parts > 1 ? seg : 0), part_b = g.b_parts > 1 ? seg : 0;
+        for (int k0 = 0; k0 < g.k_blocks * FF_BK; k0 += FF_BK) {
+          ok = __all_sync(0xffffffffu, mbar_wait(empty + s, phase) && *abort_flag == 0);
+          if (!ok) break;
+          if (elect_one()) {
+            if (rank == 0) mbar_expect_tx(full + s, CG * L::STAGE);
+            const uint32_t bar = CG == 2 ? map_rank(full + s, 0) : smem_u32(full + s);
+            uint8_t* stage = smem + s * L::STAGE;
 #pragma unroll
-        for (int q = 0; q < S; ++q) {
-          uint8_t* dA = stage + q * L::A_TILE;
-          uint8_t* dB = stage + S * L::A_TILE + q * L::B_TILE;
-          const int pa = q * g.a_parts + (g.m_parts > 1 ? m_part : (g.a_parts > 1 ? seg : 0));
-          if (!g.a_mn) {
-            tma_load_3d<CG>(dA, &g.a, bar, k0, m0, pa);
-          } else {
+            for (int q = 0; q < S; ++q) {
+              uint8_t* dA = stage + q * L::A_TILE;
+              uint8_t* dB = stage + S * L::A_TILE + q * L::B_TILE;
+              const int pa = q * g.a_parts + part_a;
+              if (!g.a_mn) {
+                tma_load_3d<CG>(dA, &g.a, bar, k0, m0, pa);
+              } else {
 #pragma unroll
-            for (int j = 0; j < FF_BM / 64; ++j) tma_load_3d<CG>(dA + j * 8192, &g.a, bar, m0 + 64 * j, k0, pa);
-          }
-          if (KIND == FF_GATE) {
-            // accumulator columns: BN / 2 gate, then BN / 2 up; of a pair, one CTA fetches the gate rows, the other the up rows
-            if (CG == 2) {
-              tma_load_3d<CG>(dB, &g.b, bar, k0, n0, q * 2 + (int)rank);
-            } else {
-              tma_load_3d<CG>(dB, &g.b, bar, k0, n0, q * 2);
-              tma_load_3d<CG>(dB + L::B_TILE / 2, &g.b, bar, k0, n0, q * 2 + 1);
+                for (int j = 0; j < FF_BM / 64; ++j) tma_load_3d<CG>(dA + j * 8192, &g.a, bar, m0 + 64 * j, k0, pa);
+              }
+              if (KIND == FF_GATE) {
+                // accumulator columns: BN / 2 gate, then BN / 2 up; of a pair, one CTA fetches the gate rows, the other the up rows
+                if (CG == 2) {
+                  tma_load_3d<CG>(dB, &g.b, bar, k0, n0, q * 2 + (int)rank);
+                } else {
+                  tma_load_3d<CG>(dB, &g.b, bar, k0, n0, q * 2);
+                  tma_load_3d<CG>(dB + L::B_TILE / 2, &g.b, bar, k0, n0, q * 2 + 1);
+                }
+              } else {
+                const int pb = q * g.b_parts + part_b, nb = n0 + (int)rank * (BN / CG);
+                if (!g.b_mn) {
+                  tma_load_3d<CG>(dB, &g.b, bar, k0, nb, pb);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < BN / CG / 64; ++j) tma_load_3d<CG>(dB + j * 8192, &g.b, bar, nb + 64 * j, k0, pb);
+                }
+              }
             }
-          } else {
-            const int pb = q * g.b_parts + (g.b_parts > 1 ? seg : 0), nb = n0 + (int)rank * (BN / CG);
-            if (!g.b_mn) {
-              tma_load_3d<CG>(dB, &g.b, bar, k0, nb, pb);
-            } else {
-#pragma unroll
-              for (int j = 0; j < BN / CG / 64; ++j) tma_load_3d<CG>(dB + j * 8192, &g.b, bar, nb + 64 * j, k0, pb);
-            }
           }
+          __syncwarp();
+          ++it;
+          if (++s == L::STAGES) { s = 0; phase ^= 1; }
         }
       }
     }
     // after a wait that ran out: the copies in flight end before this CTA's shared memory is given back
-    if (!ok && rank == 0)
-      for (uint32_t j = it > L::STAGES ? it - L::STAGES : 0; j < it; ++j) mbar_wait(full + j % L::STAGES, (j / L::STAGES) & 1);
-  } else if (warp == FF_EPI + 1 && lane == 0 && rank == 0) {
+    if (!ok) {
+      *abort_flag = 1;
+      if (rank == 0)
+        for (uint32_t j = it > L::STAGES ? it - L::STAGES : 0; j < it; ++j) mbar_wait(full + j % L::STAGES, (j / L::STAGES) & 1);
+    }
+  } else if (warp == FF_EPI + 1 && rank == 0) {
     // ---------------- MMA issuer (of a pair: the leader's) ----------------
     // instruction descriptor: fp32 accumulate, operand type, majorness bits, N >> 3, M >> 4
     const uint32_t type = g.fp16 ? 0u : 1u;
     const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)g.a_mn << 15) | ((uint32_t)g.b_mn << 16) |
                            ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
     // K-major: 16 k = 32 bytes further inside the 128-byte row, 8-row groups 1024 bytes apart; MN-major: 16 k = 16 rows of
-    // 128 bytes, 8-k groups 1024 bytes apart, blocks of 64 MN elements 8192 bytes apart
-    const uint32_t a_step = g.a_mn ? 2048 : 32, b_step = g.b_mn ? 2048 : 32;
-    const uint32_t a_lbo = g.a_mn ? 8192 : 16, b_lbo = g.b_mn ? 8192 : 16;
-    uint32_t it = 0, chunk = 0;
+    // 128 bytes, 8-k groups 1024 bytes apart, blocks of 64 MN elements 8192 bytes apart.  Descriptors count in 16 bytes.
+    const uint32_t a_step = (g.a_mn ? 2048 : 32) >> 4, b_step = (g.b_mn ? 2048 : 32) >> 4;
+    const uint32_t base = smem_u32(smem);
+    const uint64_t da0 = make_desc(base, g.a_mn ? 8192 : 16, 1024), db0 = make_desc(base + S * L::A_TILE, g.b_mn ? 8192 : 16, 1024);
+    uint32_t s = 0, phase = 0, chunk = 0;
     bool ok = true;
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step) {
-      for (int i = 0; i < n_kb; ++i, ++it) {
-        const bool first = S == 3 || i == 0;
+      for (int i = 0; i < n_kb; ++i) {
         const uint32_t buf = chunk & 1;
-        if (first && chunk >= 2 && !mbar_wait_cluster(acc_empty + buf, ((chunk >> 1) - 1) & 1)) ok = false;
-        const uint32_t s = it % L::STAGES;
-        if (ok && !mbar_wait_cluster(full + s, (it / L::STAGES) & 1)) ok = false;
-        if (!ok) { *abort_flag = 1; break; }
+        // the first round of either accumulator passes at once
+        if (S == 3 || i == 0) ok = mbar_wait(acc_empty + buf, ((chunk >> 1) & 1) ^ 1);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(full + s, phase));
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t d = tmem_base + buf * BN;
-        const uint32_t a_addr = smem_u32(smem + s * L::STAGE), b_addr = a_addr + S * L::A_TILE;
-        if (S == 1) {
+        if (elect_one()) {
+          const uint32_t d = tmem_base + buf * BN;
+          const uint64_t da = da0 + s * (L::STAGE >> 4), db = db0 + s * (L::STAGE >> 4);
+          if (S == 1) {
 #pragma unroll
-          for (int k = 0; k < FF_BK / 16; ++k)
-            umma_f16<CG>(d, make_desc(a_addr + k * a_step, a_lbo, 1024), make_desc(b_addr + k * b_step, b_lbo, 1024), idesc,
-                         (i > 0 || k > 0) ? 1u : 0u);
-        } else {
-          // smallest products first: (1,3) (3,1) (2,2) (1,2) (2,1) (1,1)
-          constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
+            for (int k = 0; k < FF_BK / 16; ++k) umma_f16<CG>(d, da + k * a_step, db + k * b_step, idesc, (i > 0 || k > 0) ? 1u : 0u);
+          } else {
+            // smallest products first: (1,3) (3,1) (2,2) (1,2) (2,1) (1,1)
+            constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
 #pragma unroll
-          for (int p = 0; p < 6; ++p)
+            for (int p = 0; p < 6; ++p)
 #pragma unroll
-            for (int k = 0; k < FF_BK / 16; ++k)
-              umma_f16<CG>(d, make_desc(a_addr + PA[p] * L::A_TILE + k * a_step, a_lbo, 1024),
-                           make_desc(b_addr + PB[p] * L::B_TILE + k * b_step, b_lbo, 1024), idesc, (p > 0 || k > 0) ? 1u : 0u);
+              for (int k = 0; k < FF_BK / 16; ++k)
+                umma_f16<CG>(d, da + PA[p] * (L::A_TILE >> 4) + k * a_step, db + PB[p] * (L::B_TILE >> 4) + k * b_step, idesc,
+                             (p > 0 || k > 0) ? 1u : 0u);
+          }
+          ff_commit<CG>(empty + s);  // frees this stage once the MMAs above have read it
+          if (S == 3 || i == n_kb - 1) ff_commit<CG>(acc_full + buf);
         }
-        ff_commit<CG>(empty + s);  // frees this stage once the MMAs above have read it
-        if (S == 3 || i == n_kb - 1) {
-          ff_commit<CG>(acc_full + buf);
-          ++chunk;
-        }
+        __syncwarp();
+        if (S == 3 || i == n_kb - 1) ++chunk;
+        if (++s == L::STAGES) { s = 0; phase ^= 1; }
       }
     }
+    if (!ok) *abort_flag = 1;
   } else if (warp < FF_EPI) {
     // ---------------- epilogue: warp w reads lanes 32 (w % 4) ... of half of the tile's output columns ----------------
     constexpr int HC = BN_OUT / 2;         // output columns per warp
@@ -492,8 +508,9 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
     uint32_t chunk = 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     for (int tile = first_tile; tile < n_tiles; tile += tile_step) {
-      const int tm = tile % (tiles_m * g.m_parts), n0 = (tile / (tiles_m * g.m_parts)) * BN_OUT + half * HC;
-      const int m_part = tm / tiles_m, row = (tm % tiles_m) * TM + (int)rank * FF_BM + (warp & 3) * 32 + lane;
+      int tm, tn;
+      ff_tile(tile, tiles_m * g.m_parts, tiles_n, tm, tn);
+      const int n0 = tn * BN_OUT + half * HC, m_part = tm / tiles_m, row = (tm % tiles_m) * TM + (int)rank * FF_BM + (warp & 3) * 32 + lane;
       bool stop = false;
       if (S == 3) {
         // the accumulator of every 64 k, added up in registers
@@ -503,7 +520,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
         for (int c = 0; c < NA; ++c) acc[c] = 0.f;
         for (int i = 0; i < n_kb; ++i, ++chunk) {
           const uint32_t buf = chunk & 1;
-          const bool bad = !mbar_wait_cluster(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
+          const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
           if (ff_epi_bar_or(bad)) { stop = true; break; }
           tc_fence_after();
 #pragma unroll
@@ -534,7 +551,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
       } else {
         const uint32_t buf = chunk & 1;
         constexpr int CH = KIND == FF_DGATE && HC >= 32 ? 32 : 16;     // dgate: 16 loads of 32 bytes in flight per thread
-        const bool bad = !mbar_wait_cluster(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
+        const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
         if (ff_epi_bar_or(bad)) stop = true;
         else {
           tc_fence_after();
