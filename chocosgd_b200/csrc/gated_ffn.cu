@@ -30,13 +30,14 @@
 #include "vec.cuh"
 
 #define FF_BM 128            // accumulator rows of one CTA
-#define FF_BK 64             // k per stage: 128 bytes of 16-bit operands = one swizzle row
+#define FF_BK(S) ((S) == 3 ? 32 : 64)    // k per stage: K-major rows of 64 (three planes) or 128 bytes = one swizzle row
 #define FF_EPI 8             // epilogue warps 0-7 (warp 0 owns TMEM), warp 8 TMA, warp 9 MMA
 #define FF_THREADS (32 * (FF_EPI + 2))
 
 #define FF_GATE 0
 #define FF_DGATE 1
 #define FF_PLAIN 2
+#define FF_PARTIAL 3         // plain, over a part of k, into fp32 slices that ffn_join_kernel adds up
 
 #define ACT_SILU 0
 #define ACT_GELU 1
@@ -48,20 +49,27 @@ __device__ int g_ffn_error;
 struct FfnGemm {
   CUtensorMap a, b;
   int M, N;              // output rows (of one part) and columns; gate: N = F
-  int k_blocks;          // 64-wide k-blocks of one segment
+  int k_blocks;          // k-blocks (FF_BK) of one segment
+  int k_splits;          // partial: slices of the k-blocks, one tile each
   int segments;          // dX: 2 (gate and up rows of W_in); else 1
   int m_parts;           // dW_in: 2 (dG and dU); else 1
   int a_parts, b_parts;  // planes per split of the operand (2: gate / up)
   int a_mn, b_mn;        // operand lies MN-major
   int fp16;              // operand type: fp16 instead of bf16 (S = 1)
   int act;
-  void* out;             // plain: [m_parts M, N];  gate: H [S][M][ldo];  dgate: dZ [S][2][M][ldo]
-  int out_dt;            // plain: type of out
-  int vec_bytes;         // plain: common alignment of out's rows (32, 16 or less)
+  void* out;             // plain: [m_parts M, N] of the operands' type;  gate: H [S][M][ldo];  dgate: dZ [S][2][M][ldo]
+  int vec16;             // out's rows start on 16-byte boundaries
   long long ldo;
-  float* z;              // gate: written (null in evaluation);  dgate: read;  [2][M][ldz]
-  long long ldz;
+  float* z;              // lane-blocked fp32 (lane_off), ldz columns.  gate: [2] G, U written (null in evaluation);
+  long long ldz;         // dgate: read;  partial: [k_splits][m_parts] written
+  long long z_plane;     // floats of one matrix of z
 };
+
+// fp32 matrices that only these kernels read (G, U, partial sums) are stored in the order in which a warp of the epilogue
+// holds them: 32 rows x 8 columns = 1 KB, 32 bytes per lane.  Row-major, a warp's access would touch 32 lines for 1 KB.
+__host__ __device__ __forceinline__ long long lane_off(int row, int col, long long ld) {
+  return (((long long)(row >> 5) * (ld >> 3) + (col >> 3)) * 32 + (row & 31)) * 8;
+}
 
 // ---- pairs of CTAs (cta_group::2) ----------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -189,21 +197,23 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int fp16) {
   return *reinterpret_cast<const uint32_t*>(&q);
 }
 
-// x as three bf16 numbers (finite x whose rounding would overflow is cut instead; the remainders of a non-finite x are zero)
-__device__ __forceinline__ void split3(float x, float (&p)[3]) {
-  p[0] = __bfloat162float(__float2bfloat16_rn(x));
-  if (!isfinite(p[0])) p[0] = __bfloat162float(__float2bfloat16_rz(x));
-  float r = x - p[0];
-  if (!isfinite(r)) r = 0.f;
-  p[1] = __bfloat162float(__float2bfloat16_rn(r));
-  p[2] = r - p[1];
+// two fp32 numbers as three pairs of bf16 numbers, each the rounded remainder of the ones before.  The first is limited to
+// the largest bf16 number, so that fp32 numbers above it keep a finite split; non-finite numbers stay non-finite.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&q)[3]) {
+  const float big = __uint_as_float(0x7F7F0000u);
+#pragma unroll
+  for (int s = 0; s < 3; ++s) {
+    q[s] = s == 0 ? pack2(fminf(fmaxf(x, -big), big), fminf(fmaxf(y, -big), big), 0) : pack2(x, y, 0);
+    x -= __uint_as_float(q[s] << 16);
+    y -= __uint_as_float(q[s] & 0xFFFF0000u);
+  }
 }
 
-// activation and (wanted) its derivative; FAST: 16-bit results, for which the approximate exponential and quotient
-// (relative error about 2^-21) are exact enough
-template <bool GRAD, bool FAST>
-__device__ __forceinline__ float ff_act(int act, float z, float& slope) {
-  if (act == ACT_GELU) {
+// activation and (wanted) its derivative.  The quotient is the approximate one (2 units of the last place); FAST: so is the
+// exponential (relative error |z| 2^-23), which suits 16-bit results.
+template <int ACT, bool GRAD, bool FAST>
+__device__ __forceinline__ float ff_act(float z, float& slope) {
+  if (ACT == ACT_GELU) {
     const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
     if (GRAD) {
       const float e = -0.5f * z * z;
@@ -211,13 +221,13 @@ __device__ __forceinline__ float ff_act(int act, float z, float& slope) {
     }
     return z * cdf;
   }
-  if (act == ACT_RELU) {
+  if (ACT == ACT_RELU) {
     if (GRAD) slope = z > 0.f ? 1.f : 0.f;
     return z < 0.f ? 0.f : z;
   }
   // __fdividef gives 0 for divisors above 2^126, which is the limit wanted here
-  const float sg = FAST ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
-  if (act == ACT_SILU) {
+  const float sg = __fdividef(1.f, 1.f + (FAST ? __expf(-z) : expf(-z)));
+  if (ACT == ACT_SILU) {
     if (GRAD) slope = sg * fmaf(z, 1.f - sg, 1.f);
     return z * sg;
   }
@@ -225,129 +235,202 @@ __device__ __forceinline__ float ff_act(int act, float z, float& slope) {
   return sg;
 }
 
-// sixteen consecutive values of one row into a 16-bit operand buffer (S planes); rows are padded to multiples of sixteen
-template <int S>
-__device__ __forceinline__ void ff_store_operand(uint16_t* base, long long plane, long long off, int fp16, const float* v) {
-  if (S == 3) {
-    uint32_t q[3][8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float lo[3], hi[3];
-      split3(v[2 * e], lo);
-      split3(v[2 * e + 1], hi);
-#pragma unroll
-      for (int s = 0; s < 3; ++s) q[s][e] = pack2(lo[s], hi[s], 0);
-    }
-#pragma unroll
-    for (int s = 0; s < 3; ++s) st32b(base + s * plane + off, q[s]);
-  } else {
-    uint32_t q[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = pack2(v[2 * e], v[2 * e + 1], fp16);
-    st32b(base + off, q);
-  }
+// ---- a warp's 32 rows x up to 128 bytes through shared memory, so that rows are written as whole lines -----------------
+// 16-byte unit c of row r lies at unit c ^ (r & 7) of the row's 128 bytes
+__device__ __forceinline__ void stage_put(uint8_t* stage, int lane, int unit, uint4 v) {
+  *reinterpret_cast<uint4*>(stage + lane * 128 + ((unit ^ (lane & 7)) << 4)) = v;
 }
-// n <= 16 of sixteen values to a row of the result; `bytes`: common alignment of its rows
-template <typename T>
-__device__ __forceinline__ void ff_store_plain(T* out, int n, int bytes, const float* v) {
-  constexpr int W = 16 / (int)sizeof(T);
-  if (n >= 16 && bytes >= 32) {
+__device__ __forceinline__ uint4 stage_get(const uint8_t* stage, int row, int unit) {
+  return *reinterpret_cast<const uint4*>(stage + row * 128 + ((unit ^ (row & 7)) << 4));
+}
+// UNITS 16-byte units per row, from unit `u0`, to rows [0, rows) of `out` (ES bytes per element, ld elements per row), of
+// which `cols` elements exist.  vec16: rows start on 16-byte boundaries.  Called by whole warps.
+template <int UNITS, int ES>
+__device__ __forceinline__ void stage_flush(const uint8_t* stage, int u0, uint8_t* out, long long ld, int rows, int cols,
+                                            int vec16, int lane) {
+  constexpr int EU = 16 / ES;      // elements per unit
+  if (vec16) {
 #pragma unroll
-    for (int h = 0; h < 16; h += 2 * W) {
-      union { T e[2 * W]; uint32_t r[8]; } q;
+    for (int i = 0; i < UNITS; ++i) {
+      const int r = (i * 32 + lane) / UNITS, c = (i * 32 + lane) % UNITS;
+      if (r < rows && c * EU < cols) {
+        const uint4 v = stage_get(stage, r, u0 + c);
+        uint8_t* p = out + ((long long)r * ld + c * EU) * ES;
+        if (c * EU + EU <= cols) {
+          *reinterpret_cast<uint4*>(p) = v;
+        } else {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < 2 * W; ++e) q.e[e] = from_f<T>(v[h + e]);
-      st32b(out + h, q.r);
-    }
-    return;
-  }
-  if (bytes >= 16) {
-#pragma unroll
-    for (int h = 0; h < 16; h += W) {
-      if (h + W <= n) {
-        Vec<T, W> q;
-#pragma unroll
-        for (int e = 0; e < W; ++e) q.e[e] = from_f<T>(v[h + e]);
-        q.store(out + h);
-      } else {
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          if (h + e < n) out[h + e] = from_f<T>(v[h + e]);
+          for (int e = 0; e < EU; ++e)
+            if (c * EU + e < cols) {
+              if (ES == 4) reinterpret_cast<uint32_t*>(p)[e] = w[e & 3];
+              else reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            }
+        }
       }
     }
-    return;
-  }
+  } else {
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e)
-    if (e < n) out[e] = from_f<T>(v[e]);
+      for (int e = lane; e < UNITS * EU; e += 32)
+        if (e < cols) {
+          const uint8_t* src = stage + r * 128 + (((u0 + e / EU) ^ (r & 7)) << 4) + (e % EU) * ES;
+          uint8_t* p = out + ((long long)r * ld + e) * ES;
+          if (ES == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(src);
+          else *reinterpret_cast<uint16_t*>(p) = *reinterpret_cast<const uint16_t*>(src);
+        }
+    }
+  }
 }
 
-// The epilogue of columns [col, col + 16) of one row: v = accumulator (gate: G in v, U in u; dgate: G and U of the forward
-// pass in zg, zu).  Buffers between the products have rows padded to sixteen elements: whole runs are written there.
-template <int S, int KIND>
-__device__ __forceinline__ void ff_epilogue16(const FfnGemm& g, int m_part, int row, int col, const float* v, const float* u,
-                                              const float* zg, const float* zu) {
-  constexpr bool FAST = S == 1;
-  if (KIND == FF_GATE) {
-    if (g.z != nullptr) {
-      float* z = g.z + (long long)row * g.ldz + col;
-      st32b(z, reinterpret_cast<const uint32_t*>(v));
-      st32b(z + 8, reinterpret_cast<const uint32_t*>(v + 8));
-      z += (long long)g.M * g.ldz;
-      st32b(z, reinterpret_cast<const uint32_t*>(u));
-      st32b(z + 8, reinterpret_cast<const uint32_t*>(u + 8));
-    }
-    float h[16], slope;
+// What a warp does with its 32 rows x HC output columns of a tile, sixteen columns at a time: put() for each, in order.
+// v = accumulator (gate: G in v, U in u; dgate: dH, with G and U in zg, zu).  Buffers between the products have rows padded
+// to sixteen elements and are written in whole runs.
+template <int S, int KIND, int HC, int ACT> struct FfnEpilogue {
+  const FfnGemm& g;
+  uint8_t* stage;
+  int m_part, row0, col0, lane;      // first row and column of the warp
+
+  __device__ __forceinline__ void put(int c, const float* v, const float* u, const float* zg, const float* zu) {
+    constexpr bool FAST = S == 1;
+    const int col = col0 + c;
+    if (KIND == FF_GATE) {
+      float h[16], slope;
+      if (g.z != nullptr && row0 < g.M && col < g.N) {
+        float* z = g.z + lane_off(row0 + lane, col, g.ldz);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) h[e] = ff_act<false, FAST>(g.act, v[e], slope) * u[e];
-    ff_store_operand<S>(reinterpret_cast<uint16_t*>(g.out), (long long)g.M * g.ldo, (long long)row * g.ldo + col, g.fp16, h);
-  } else if (KIND == FF_DGATE) {
-    float dg[16], du[16];
+        for (int k = 0; k < 2; ++k) {
+          st32b(z + k * 256, reinterpret_cast<const uint32_t*>(v + 8 * k));
+          st32b(z + k * 256 + g.z_plane, reinterpret_cast<const uint32_t*>(u + 8 * k));
+        }
+      }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float slope;
-      const float a = ff_act<true, FAST>(g.act, zg[e], slope);
-      du[e] = v[e] * a;
-      dg[e] = v[e] * zu[e] * slope;
+      for (int e = 0; e < 16; ++e) h[e] = ff_act<ACT, false, FAST>(v[e], slope) * u[e];
+      operand<(HC < 64 ? HC : 64)>(c, 0, h, 0, g.M * g.ldo);
+    } else if (KIND == FF_DGATE) {
+      float dg[16], du[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float slope;
+        const float a = ff_act<ACT, true, FAST>(zg[e], slope);
+        du[e] = v[e] * a;
+        dg[e] = v[e] * zu[e] * slope;
+      }
+      const long long plane = g.M * g.ldo;
+      operand<(HC < 32 ? HC : 32)>(c, 0, dg, 0, 2 * plane);
+      operand<(HC < 32 ? HC : 32)>(c, 4, du, plane, 2 * plane);
+    } else if (KIND == FF_PARTIAL) {
+      if (row0 < g.M && col < g.N) {
+        float* z = g.z + m_part * g.z_plane + lane_off(row0 + lane, col, g.ldz);
+        st32b(z, reinterpret_cast<const uint32_t*>(v));
+        st32b(z + 256, reinterpret_cast<const uint32_t*>(v + 8));
+      }
+    } else if (S == 3) {
+      constexpr int FC = HC < 32 ? HC : 32;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        stage_put(stage, lane, c % FC / 4 + k, make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
+                                                          __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])));
+      if ((c + 16) % FC == 0) flush<FC / 4, 4>(c + 16 - FC, 0, (long long)m_part * g.M * g.ldo, g.N);
+    } else {
+      constexpr int FC = HC < 64 ? HC : 64;
+      pack16(c % FC / 8, v);
+      if ((c + 16) % FC == 0) flush<FC / 8, 2>(c + 16 - FC, 0, (long long)m_part * g.M * g.ldo, g.N);
     }
-    const long long plane = (long long)g.M * g.ldo, off = (long long)row * g.ldo + col;
-    ff_store_operand<S>(reinterpret_cast<uint16_t*>(g.out), 2 * plane, off, g.fp16, dg);
-    ff_store_operand<S>(reinterpret_cast<uint16_t*>(g.out), 2 * plane, plane + off, g.fp16, du);
-  } else {
-    const long long off = ((long long)m_part * g.M + row) * g.ldo + col;
-    const int n = g.N - col;
-    if (g.out_dt == DT_F32) ff_store_plain(reinterpret_cast<float*>(g.out) + off, n, g.vec_bytes, v);
-    else if (g.out_dt == DT_BF16) ff_store_plain(reinterpret_cast<__nv_bfloat16*>(g.out) + off, n, g.vec_bytes, v);
-    else ff_store_plain(reinterpret_cast<__half*>(g.out) + off, n, g.vec_bytes, v);
   }
-}
-// G and U of sixteen columns (dgate)
-__device__ __forceinline__ void ff_load_z(const FfnGemm& g, int row, int col, float* zg, float* zu) {
-  const float* z = g.z + (long long)row * g.ldz + col;
-  ld32b(z, reinterpret_cast<uint32_t*>(zg));
-  ld32b(z + 8, reinterpret_cast<uint32_t*>(zg + 8));
-  z += (long long)g.M * g.ldz;
-  ld32b(z, reinterpret_cast<uint32_t*>(zu));
-  ld32b(z + 8, reinterpret_cast<uint32_t*>(zu + 8));
+  __device__ __forceinline__ void pack16(int unit, const float* v) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      stage_put(stage, lane, unit + k, make_uint4(pack2(v[8 * k], v[8 * k + 1], g.fp16), pack2(v[8 * k + 2], v[8 * k + 3], g.fp16),
+                                                  pack2(v[8 * k + 4], v[8 * k + 5], g.fp16), pack2(v[8 * k + 6], v[8 * k + 7], g.fp16)));
+  }
+  template <int UNITS, int ES>
+  __device__ __forceinline__ void flush(int c, int u0, long long off, long long cols) {
+    __syncwarp();
+    stage_flush<UNITS, ES>(stage, u0, reinterpret_cast<uint8_t*>(g.out) + (off + (long long)row0 * g.ldo + col0 + c) * ES, g.ldo,
+                           min(32, g.M - row0), (int)cols - col0 - c, g.vec16, lane);
+    __syncwarp();
+  }
+  // a 16-bit operand buffer: FC columns are gathered in shared memory (from unit u0); three planes are written directly
+  template <int FC>
+  __device__ __forceinline__ void operand(int c, int u0, const float* v, long long off, long long plane) {
+    if (S == 3) {
+      if (row0 + lane >= g.M || col0 + c >= g.ldo) return;
+      uint32_t q[3][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t p[3];
+        split3(v[2 * e], v[2 * e + 1], p);
+#pragma unroll
+        for (int s = 0; s < 3; ++s) q[s][e] = p[s];
+      }
+      uint16_t* o = reinterpret_cast<uint16_t*>(g.out) + off + (long long)(row0 + lane) * g.ldo + col0 + c;
+#pragma unroll
+      for (int s = 0; s < 3; ++s) st32b(o + s * plane, q[s]);
+    } else {
+      pack16(u0 + c % FC / 8, v);
+      if ((c + 16) % FC == 0) flush<FC / 8, 2>(c + 16 - FC, u0, off, g.ldo);
+    }
+  }
+};
+// G and U of sixteen columns of a row (dgate); zeros outside
+__device__ __forceinline__ void ff_load_z(const FfnGemm& g, int row0, int lane, int col, float* zg, float* zu) {
+  if (row0 < g.M && col < g.N) {
+    const float* z = g.z + lane_off(row0 + lane, col, g.ldz);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      ld32b(z + k * 256, reinterpret_cast<uint32_t*>(zg + 8 * k));
+      ld32b(z + k * 256 + g.z_plane, reinterpret_cast<uint32_t*>(zu + 8 * k));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) zg[e] = zu[e] = 0.f;
+  }
 }
 
 // BN accumulator columns, S operand planes, CG CTAs per tile: a pair (CG = 2) shares one 256-row tile, each CTA fetches its
 // 128 rows of A and half of the B tile, so a byte of B serves 256 rows
 template <int BN, int S, int CG> struct FfnSmem {
-  static constexpr int A_TILE = FF_BM * FF_BK * 2, B_TILE = BN / CG * FF_BK * 2;
+  static constexpr int A_TILE = FF_BM * FF_BK(S) * 2, B_TILE = BN / CG * FF_BK(S) * 2;
   static constexpr int STAGE = S * (A_TILE + B_TILE);
-  static constexpr int STAGES = (216 * 1024) / STAGE > 8 ? 8 : (216 * 1024) / STAGE;
-  static constexpr int BYTES = STAGES * STAGE + 256 + 1024;
+  static constexpr int EPI = FF_EPI * 4096;               // 4 KB for each epilogue warp
+  static constexpr int ROOM = 227 * 1024 - 256 - 1024 - EPI;
+  static constexpr int STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
+  static constexpr int BYTES = STAGES * STAGE + EPI + 256 + 1024;
 };
 
 // Tile order: groups of FF_GROUP row tiles, rows fastest within a group, so that the tiles worked on at one time form a
 // block that is about as high as wide and share both operands' panels in L2.
 #define FF_GROUP 8
-__device__ __forceinline__ void ff_tile(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+__device__ __forceinline__ void ff_tile(int tile, int out_tiles, int tiles_m, int tiles_n, int& tm, int& tn) {
+  tile %= out_tiles;
   const int per_group = FF_GROUP * tiles_n, group = tile / per_group, r = tile - group * per_group;
   const int rows = min(FF_GROUP, tiles_m - group * FF_GROUP);
   tn = r / rows;
   tm = group * FF_GROUP + (r - tn * rows);
+}
+
+// f(the activation as a constant): the choice is made once per tile, so that the code that runs stays small
+template <int V> struct FfnConst { static constexpr int value = V; };
+template <int KIND, typename F>
+__device__ __forceinline__ void ff_for_act(int act, F f) {
+  if (KIND == FF_PLAIN || KIND == FF_PARTIAL || act == ACT_SILU) f(FfnConst<ACT_SILU>());
+  else if (act == ACT_GELU) f(FfnConst<ACT_GELU>());
+  else if (act == ACT_RELU) f(FfnConst<ACT_RELU>());
+  else f(FfnConst<ACT_SIGMOID>());
+}
+
+// k-blocks [kb0, kb1) of a tile
+template <int KIND>
+__device__ __forceinline__ void ff_slice(const FfnGemm& g, int tile, int out_tiles, int n_kb, int& kb0, int& kb1) {
+  kb0 = 0;
+  kb1 = n_kb;
+  if (KIND == FF_PARTIAL) {
+    const int q = tile / out_tiles;
+    kb0 = (int)((long long)n_kb * q / g.k_splits);
+    kb1 = (int)((long long)n_kb * (q + 1) / g.k_splits);
+  }
 }
 
 template <int BN, int S, int KIND, int CG>
@@ -356,7 +439,9 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
   extern __shared__ uint8_t smem_raw[];
   // 1024-byte alignment: the swizzle pattern is a function of the shared-memory address bits
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::STAGES * L::STAGE);   // CG = 2: the leader's count both CTAs' bytes
+  constexpr int BK = FF_BK(S), CHUNK = 64 / BK;     // S = 3: an accumulator holds 64 k
+  uint8_t* epi_smem = smem + L::STAGES * L::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi_smem + L::EPI);   // CG = 2: the leader's count both CTAs' bytes
   uint64_t* empty = full + L::STAGES;
   uint64_t* acc_full = empty + L::STAGES;    // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2], the leader's
@@ -368,8 +453,9 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   const int tiles_m = (g.M + TM - 1) / TM, tiles_n = (g.N + BN_OUT - 1) / BN_OUT;
-  const int n_tiles = tiles_m * g.m_parts * tiles_n;
-  const int n_kb = g.k_blocks * g.segments;
+  const int out_tiles = tiles_m * g.m_parts * tiles_n;
+  const int n_tiles = KIND == FF_PARTIAL ? out_tiles * g.k_splits : out_tiles;
+  const int n_kb_all = g.k_blocks * g.segments;
   const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
 
   if (threadIdx.x == 0) {
@@ -401,12 +487,14 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
     uint32_t it = 0, s = 0, phase = 1;      // stage and the parity of its `empty` barrier (the first round passes at once)
     bool ok = true;
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step) {
-      int tm, tn;
-      ff_tile(tile, tiles_m * g.m_parts, tiles_n, tm, tn);
+      int tm, tn, kb0, kb1;
+      ff_slice<KIND>(g, tile, out_tiles, n_kb_all, kb0, kb1);
+      ff_tile(tile, out_tiles, tiles_m * g.m_parts, tiles_n, tm, tn);
       const int n0 = tn * BN_OUT, m_part = tm / tiles_m, m0 = (tm % tiles_m) * TM + (int)rank * FF_BM;
-      for (int seg = 0; seg < g.segments && ok; ++seg) {
-        const int part_a = g.m_parts > 1 ? m_part : (g.a_parts > 1 ? seg : 0), part_b = g.b_parts > 1 ? seg : 0;
-        for (int k0 = 0; k0 < g.k_blocks * FF_BK; k0 += FF_BK) {
+      {
+        for (int i = kb0; i < kb1; ++i) {
+          const int seg = i >= g.k_blocks ? 1 : 0, k0 = (i - seg * g.k_blocks) * BK;
+          const int part_a = g.m_parts > 1 ? m_part : (g.a_parts > 1 ? seg : 0), part_b = g.b_parts > 1 ? seg : 0;
           ok = __all_sync(0xffffffffu, mbar_wait(empty + s, phase) && *abort_flag == 0);
           if (!ok) break;
           if (elect_one()) {
@@ -422,7 +510,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
                 tma_load_3d<CG>(dA, &g.a, bar, k0, m0, pa);
               } else {
 #pragma unroll
-                for (int j = 0; j < FF_BM / 64; ++j) tma_load_3d<CG>(dA + j * 8192, &g.a, bar, m0 + 64 * j, k0, pa);
+                for (int j = 0; j < FF_BM / 64; ++j) tma_load_3d<CG>(dA + j * BK * 128, &g.a, bar, m0 + 64 * j, k0, pa);
               }
               if (KIND == FF_GATE) {
                 // accumulator columns: BN / 2 gate, then BN / 2 up; of a pair, one CTA fetches the gate rows, the other the up rows
@@ -438,7 +526,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
                   tma_load_3d<CG>(dB, &g.b, bar, k0, nb, pb);
                 } else {
 #pragma unroll
-                  for (int j = 0; j < BN / CG / 64; ++j) tma_load_3d<CG>(dB + j * 8192, &g.b, bar, nb + 64 * j, k0, pb);
+                  for (int j = 0; j < BN / CG / 64; ++j) tma_load_3d<CG>(dB + j * BK * 128, &g.b, bar, nb + 64 * j, k0, pb);
                 }
               }
             }
@@ -461,18 +549,24 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
     const uint32_t type = g.fp16 ? 0u : 1u;
     const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)g.a_mn << 15) | ((uint32_t)g.b_mn << 16) |
                            ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
-    // K-major: 16 k = 32 bytes further inside the 128-byte row, 8-row groups 1024 bytes apart; MN-major: 16 k = 16 rows of
-    // 128 bytes, 8-k groups 1024 bytes apart, blocks of 64 MN elements 8192 bytes apart.  Descriptors count in 16 bytes.
+    // K-major: 16 k = 32 bytes further inside the (64- or 128-byte) row, groups of 8 rows apart; MN-major: 16 k = 16 rows of
+    // 128 bytes, 8-k groups 1024 bytes apart, blocks of 64 MN elements BK rows apart.  Descriptors count in 16 bytes.
     const uint32_t a_step = (g.a_mn ? 2048 : 32) >> 4, b_step = (g.b_mn ? 2048 : 32) >> 4;
     const uint32_t base = smem_u32(smem);
-    const uint64_t da0 = make_desc(base, g.a_mn ? 8192 : 16, 1024), db0 = make_desc(base + S * L::A_TILE, g.b_mn ? 8192 : 16, 1024);
+    const uint64_t da0 = g.a_mn ? make_desc(base, BK * 128, 1024) : make_desc(base, 16, BK * 16, BK == 32 ? 4 : 2);
+    const uint64_t db0 = g.b_mn ? make_desc(base + S * L::A_TILE, BK * 128, 1024)
+                                : make_desc(base + S * L::A_TILE, 16, BK * 16, BK == 32 ? 4 : 2);
     uint32_t s = 0, phase = 0, chunk = 0;
     bool ok = true;
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step) {
+      int kb0, kb1;
+      ff_slice<KIND>(g, tile, out_tiles, n_kb_all, kb0, kb1);
+      const int n_kb = kb1 - kb0;
       for (int i = 0; i < n_kb; ++i) {
         const uint32_t buf = chunk & 1;
+        const bool first = S == 3 ? i % CHUNK == 0 : i == 0, last = (S == 3 && i % CHUNK == CHUNK - 1) || i == n_kb - 1;
         // the first round of either accumulator passes at once
-        if (S == 3 || i == 0) ok = mbar_wait(acc_empty + buf, ((chunk >> 1) & 1) ^ 1);
+        if (first) ok = mbar_wait(acc_empty + buf, ((chunk >> 1) & 1) ^ 1);
         ok = __all_sync(0xffffffffu, ok && mbar_wait(full + s, phase));
         if (!ok) break;
         tc_fence_after();
@@ -481,22 +575,22 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
           const uint64_t da = da0 + s * (L::STAGE >> 4), db = db0 + s * (L::STAGE >> 4);
           if (S == 1) {
 #pragma unroll
-            for (int k = 0; k < FF_BK / 16; ++k) umma_f16<CG>(d, da + k * a_step, db + k * b_step, idesc, (i > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) umma_f16<CG>(d, da + k * a_step, db + k * b_step, idesc, (!first || k > 0) ? 1u : 0u);
           } else {
             // smallest products first: (1,3) (3,1) (2,2) (1,2) (2,1) (1,1)
             constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
 #pragma unroll
             for (int p = 0; p < 6; ++p)
 #pragma unroll
-              for (int k = 0; k < FF_BK / 16; ++k)
+              for (int k = 0; k < BK / 16; ++k)
                 umma_f16<CG>(d, da + PA[p] * (L::A_TILE >> 4) + k * a_step, db + PB[p] * (L::B_TILE >> 4) + k * b_step, idesc,
-                             (p > 0 || k > 0) ? 1u : 0u);
+                             (!first || p > 0 || k > 0) ? 1u : 0u);
           }
           ff_commit<CG>(empty + s);  // frees this stage once the MMAs above have read it
-          if (S == 3 || i == n_kb - 1) ff_commit<CG>(acc_full + buf);
+          if (last) ff_commit<CG>(acc_full + buf);
         }
         __syncwarp();
-        if (S == 3 || i == n_kb - 1) ++chunk;
+        if (last) ++chunk;
         if (++s == L::STAGES) { s = 0; phase ^= 1; }
       }
     }
@@ -508,29 +602,37 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
     uint32_t chunk = 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     for (int tile = first_tile; tile < n_tiles; tile += tile_step) {
-      int tm, tn;
-      ff_tile(tile, tiles_m * g.m_parts, tiles_n, tm, tn);
-      const int n0 = tn * BN_OUT + half * HC, m_part = tm / tiles_m, row = (tm % tiles_m) * TM + (int)rank * FF_BM + (warp & 3) * 32 + lane;
+      int tm, tn, kb0, kb1;
+      ff_slice<KIND>(g, tile, out_tiles, n_kb_all, kb0, kb1);
+      ff_tile(tile, out_tiles, tiles_m * g.m_parts, tiles_n, tm, tn);
+      const int m_part = tm / tiles_m;
+      const int z_index = KIND == FF_PARTIAL ? tile / out_tiles * g.m_parts + m_part : m_part;
+      const int row0 = (tm % tiles_m) * TM + (int)rank * FF_BM + (warp & 3) * 32, col0 = tn * BN_OUT + half * HC;
       bool stop = false;
       if (S == 3) {
-        // the accumulator of every 64 k, added up in registers
+        // the accumulators of every 64 k, added up in registers
         constexpr int NA = KIND == FF_GATE ? 2 * HC : HC;
+        const int n_chunks = (kb1 - kb0 + CHUNK - 1) / CHUNK;
         float acc[NA];
 #pragma unroll
         for (int c = 0; c < NA; ++c) acc[c] = 0.f;
-        for (int i = 0; i < n_kb; ++i, ++chunk) {
+        for (int i = 0; i < n_chunks; ++i, ++chunk) {
           const uint32_t buf = chunk & 1;
           const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
           if (ff_epi_bar_or(bad)) { stop = true; break; }
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < NA; c += 16) {
-            float v[16];
-            const int col = c < HC ? half * HC + c : BN_OUT + half * HC + c - HC;
-            tmem_ld16_async(tmem_base + lanes + buf * BN + col, v);
-            tmem_wait16(v);
+          for (int c = 0; c < NA; c += 32) {
+            float v[32];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[c + e] += v[e];
+            for (int e = 0; e < 32 && c + e < NA; e += 16) {
+              const int col = c + e < HC ? half * HC + c + e : BN_OUT + half * HC + c + e - HC;
+              tmem_ld16_async(tmem_base + lanes + buf * BN + col, v + e);
+            }
+#pragma unroll
+            for (int e = 0; e < 32 && c + e < NA; e += 16) tmem_wait16(v + e);
+#pragma unroll
+            for (int e = 0; e < 32 && c + e < NA; ++e) acc[c + e] += v[e];
           }
           tc_fence_before();
           __syncwarp();
@@ -539,42 +641,48 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
             else mbar_arrive(acc_empty + buf);
           }
         }
-        if (!stop && row < g.M) {
+        if (!stop) {
+          ff_for_act<KIND>(g.act, [&](auto act) {
+            FfnEpilogue<S, KIND, HC, decltype(act)::value> epi = {g, epi_smem + warp * 4096, z_index, row0, col0, lane};
+            float zg[16], zu[16];
 #pragma unroll
-          for (int c = 0; c < HC; c += 16)
-            if (n0 + c < g.N) {
-              float zg[16], zu[16];
-              if (KIND == FF_DGATE) ff_load_z(g, row, n0 + c, zg, zu);
-              ff_epilogue16<S, KIND>(g, m_part, row, n0 + c, acc + c, acc + (KIND == FF_GATE ? HC + c : c), zg, zu);
+            for (int c = 0; c < HC; c += 16) {
+              if (KIND == FF_DGATE) ff_load_z(g, row0, lane, col0 + c, zg, zu);
+              epi.put(c, acc + c, acc + (KIND == FF_GATE ? HC + c : c), zg, zu);
             }
+          });
         }
       } else {
         const uint32_t buf = chunk & 1;
-        constexpr int CH = KIND == FF_DGATE && HC >= 32 ? 32 : 16;     // dgate: 16 loads of 32 bytes in flight per thread
+        // dgate: G and U of the next sixteen columns are under way while the present ones are worked on; the first ones
+        // while the tile is still being multiplied
+        float zg[16], zu[16], yg[16], yu[16];
+        if (KIND == FF_DGATE) ff_load_z(g, row0, lane, col0, zg, zu);
         const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
         if (ff_epi_bar_or(bad)) stop = true;
         else {
           tc_fence_after();
+          ff_for_act<KIND>(g.act, [&](auto act) {
+            FfnEpilogue<S, KIND, HC, decltype(act)::value> epi = {g, epi_smem + warp * 4096, z_index, row0, col0, lane};
+            const uint32_t acc = tmem_base + lanes + buf * BN + half * HC;
 #pragma unroll 1
-          for (int c = 0; c < HC; c += CH) {
-            float v[CH], u[16], zg[CH], zu[CH];
-            if (KIND == FF_DGATE && row < g.M) {
-#pragma unroll
-              for (int e = 0; e < CH; e += 16)
-                if (n0 + c + e < g.N) ff_load_z(g, row, n0 + c + e, zg + e, zu + e);
+            for (int c = 0; c < HC; c += 32) {
+              float v[16], u[16];
+              if (KIND == FF_DGATE && c + 16 < HC) ff_load_z(g, row0, lane, col0 + c + 16, yg, yu);
+              tmem_ld16_async(acc + c, v);
+              if (KIND == FF_GATE) tmem_ld16_async(acc + BN_OUT + c, u);
+              tmem_wait16(v);
+              if (KIND == FF_GATE) tmem_wait16(u);
+              epi.put(c, v, u, zg, zu);
+              if (HC < 32) break;
+              if (KIND == FF_DGATE && c + 32 < HC) ff_load_z(g, row0, lane, col0 + c + 32, zg, zu);
+              tmem_ld16_async(acc + c + 16, v);
+              if (KIND == FF_GATE) tmem_ld16_async(acc + BN_OUT + c + 16, u);
+              tmem_wait16(v);
+              if (KIND == FF_GATE) tmem_wait16(u);
+              epi.put(c + 16, v, u, yg, yu);
             }
-#pragma unroll
-            for (int e = 0; e < CH; e += 16) tmem_ld16_async(tmem_base + lanes + buf * BN + half * HC + c + e, v + e);
-            if (KIND == FF_GATE) tmem_ld16_async(tmem_base + lanes + buf * BN + BN_OUT + half * HC + c, u);
-#pragma unroll
-            for (int e = 0; e < CH; e += 16) tmem_wait16(v + e);
-            if (KIND == FF_GATE) tmem_wait16(u);
-            if (row < g.M) {
-#pragma unroll
-              for (int e = 0; e < CH; e += 16)
-                if (n0 + c + e < g.N) ff_epilogue16<S, KIND>(g, m_part, row, n0 + c + e, v + e, u, zg + e, zu + e);
-            }
-          }
+          });
           // the accumulator may be overwritten by the tile after next
           tc_fence_before();
           __syncwarp();
@@ -600,38 +708,108 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
 
 // ---- operands: fp32 into three bf16 planes, 16-bit rows onto 32-byte boundaries -------------------------------------
 // src [rows, cols] with lds elements per row -> dst [S][rows][ldd], ldd a multiple of sixteen; the tail columns are zero
-// (uint16_t stands for either 16-bit type: the values are moved, not read)
-__device__ __forceinline__ float to_f(uint16_t) { return 0.f; }
-template <typename T, int S>
-__global__ void __launch_bounds__(256) ffn_operand_kernel(const T* src, long long rows, int cols, long long lds, uint16_t* dst, int ldd) {
+struct FfnImage {
+  const void* src;
+  uint16_t* dst;
+  long long rows, lds;
+  int cols, ldd, vec;       // vec: elements per access that the row starts allow (1, 2, 4)
+  int first_block;          // blocks [first_block, next image's) copy this matrix
+};
+struct FfnImages {
+  FfnImage m[3];
+  int n;
+};
+#define FF_IMG_ROWS 8       // rows per block, one per warp
+#define FF_IMG_SPAN 4096    // columns per block
+template <int S>
+__global__ void __launch_bounds__(32 * FF_IMG_ROWS) ffn_operand_kernel(const __grid_constant__ FfnImages a) {
   pdl_wait();
   pdl_trigger();
-  const int per_row = ldd / 8;
-  const long long total = rows * per_row;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long r = i / per_row;
-    const int c = (int)(i - r * per_row) * 8;
-    const T* p = src + r * lds + c;
-    uint16_t* q = dst + r * ldd + c;
+  int k = 0;
+  while (k + 1 < a.n && (int)blockIdx.x >= a.m[k + 1].first_block) ++k;
+  const FfnImage& m = a.m[k];
+  const int spans = (m.ldd + FF_IMG_SPAN - 1) / FF_IMG_SPAN, b = (int)blockIdx.x - m.first_block;
+  const long long r = (long long)(b / spans) * FF_IMG_ROWS + (threadIdx.x >> 5);
+  if (r >= m.rows) return;
+  const int c_end = min(m.ldd, (b % spans + 1) * FF_IMG_SPAN);
+  for (int c = (b % spans) * FF_IMG_SPAN + (threadIdx.x & 31) * 8; c < c_end; c += 256) {
+    uint16_t* q = m.dst + r * m.ldd + c;
     if (S == 3) {
+      const float* p = reinterpret_cast<const float*>(m.src) + r * m.lds + c;
+      float v[8];
+      if (c + 8 <= m.cols && m.vec == 4) {
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
+      } else if (c + 8 <= m.cols && m.vec == 2) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(v + e) = *reinterpret_cast<const float2*>(p + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < m.cols ? p[e] : 0.f;
+      }
       uint32_t o[3][4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float lo[3], hi[3];
-        split3(c + 2 * e < cols ? to_f(p[2 * e]) : 0.f, lo);
-        split3(c + 2 * e + 1 < cols ? to_f(p[2 * e + 1]) : 0.f, hi);
+        uint32_t w[3];
+        split3(v[2 * e], v[2 * e + 1], w);
 #pragma unroll
-        for (int s = 0; s < 3; ++s) o[s][e] = pack2(lo[s], hi[s], 0);
+        for (int s = 0; s < 3; ++s) o[s][e] = w[s];
       }
 #pragma unroll
-      for (int s = 0; s < 3; ++s) *reinterpret_cast<uint4*>(q + s * rows * ldd) = make_uint4(o[s][0], o[s][1], o[s][2], o[s][3]);
+      for (int s = 0; s < 3; ++s) *reinterpret_cast<uint4*>(q + s * m.rows * m.ldd) = make_uint4(o[s][0], o[s][1], o[s][2], o[s][3]);
     } else {
-      Vec<T, 16 / sizeof(T)> v;
+      // 16-bit values are moved, not read
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(m.src) + r * m.lds + c;
+      Vec<uint16_t, 8> v;
       v.clear();
+      if (c + 8 <= m.cols && m.vec >= 2) {
+        uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 16 / (int)sizeof(T); ++e)
-        if (c + e < cols) v.e[e] = p[e];
-      v.store(reinterpret_cast<T*>(q));
+        for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint32_t*>(p + 2 * e);
+        v.raw = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < m.cols) v.e[e] = p[e];
+      }
+      v.store(q);
+    }
+  }
+}
+
+// out [m_parts M, N] = sum over k_splits slices of partial sums, in slice order; one thread per 8 columns
+template <typename T>
+__global__ void __launch_bounds__(256) ffn_join_kernel(const float* z, long long ldz, long long z_plane, int splits, int m_parts,
+                                                       int M, int N, T* out, int vec16) {
+  pdl_wait();
+  pdl_trigger();
+  const int groups = (int)(ldz >> 3), blocks = (M + 31) / 32, lane = threadIdx.x & 31;
+  const int total = m_parts * blocks * groups;      // one warp each
+  for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < total; j += gridDim.x * 8) {
+    const int rb = j / groups, col = (j - rb * groups) * 8, part = rb / blocks, row = (rb - part * blocks) * 32 + lane;
+    if (row >= M || col >= N) continue;
+    float v[8], w[8];
+    const float* p = z + part * z_plane + lane_off(row, col, ldz);
+    ld32b(p, reinterpret_cast<uint32_t*>(v));
+    for (int q = 1; q < splits; ++q) {
+      ld32b(p + (long long)q * m_parts * z_plane, reinterpret_cast<uint32_t*>(w));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += w[e];
+    }
+    T* o = out + ((long long)part * M + row) * N + col;
+    constexpr int W = 16 / (int)sizeof(T);
+    if (vec16 && col + 8 <= N) {
+#pragma unroll
+      for (int h = 0; h < 8; h += W) {
+        Vec<T, W> r;
+#pragma unroll
+        for (int e = 0; e < W; ++e) r.e[e] = from_f<T>(v[(h + e) & 7]);
+        r.store(o + h);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < N) o[e] = from_f<T>(v[e]);
     }
   }
 }
@@ -646,15 +824,16 @@ struct FfnOperand {
   long long ld;
 };
 
-static int ffn_map(CUtensorMap* map, const FfnOperand& o, int fp16, int mn_major, int box_rows) {
+static int ffn_map(CUtensorMap* map, const FfnOperand& o, int fp16, int mn_major, int box_rows, int bk) {
   TcEncodeTiledFn enc = tc_get_encode();
   if (enc == nullptr) return -10;
   if (((uintptr_t)o.p & 15) != 0 || o.ld % 8 != 0) return -11;
   cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)(o.parts * o.splits)};
   cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)o.ld * 2 * (cuuint64_t)o.rows};
-  cuuint32_t box[3] = {64, (cuuint32_t)(mn_major ? FF_BK : box_rows), 1}, es[3] = {1, 1, 1};
+  cuuint32_t box[3] = {(cuuint32_t)(mn_major ? 64 : bk), (cuuint32_t)(mn_major ? bk : box_rows), 1}, es[3] = {1, 1, 1};
   CUresult r = enc(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p),
-                   dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   !mn_major && bk == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -12;
 }
@@ -667,12 +846,13 @@ static int ffn_launch_t(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cu
   // (autograd's), without which the driver refuses to encode a map
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
-  int rc = ffn_map(&g.a, a, g.fp16, g.a_mn, FF_BM);
+  int rc = ffn_map(&g.a, a, g.fp16, g.a_mn, FF_BM, FF_BK(S));
   if (rc) return rc;
-  rc = ffn_map(&g.b, b, g.fp16, g.b_mn, KIND == FF_GATE ? BN / 2 : BN / CG);
+  rc = ffn_map(&g.b, b, g.fp16, g.b_mn, KIND == FF_GATE ? BN / 2 : BN / CG, FF_BK(S));
   if (rc) return rc;
   const int bn_out = KIND == FF_GATE ? BN / 2 : BN;
-  const long long tiles = (long long)((g.M + CG * FF_BM - 1) / (CG * FF_BM)) * g.m_parts * ((g.N + bn_out - 1) / bn_out);
+  const long long tiles = (long long)((g.M + CG * FF_BM - 1) / (CG * FF_BM)) * g.m_parts * ((g.N + bn_out - 1) / bn_out) *
+                          (KIND == FF_PARTIAL ? g.k_splits : 1);
   if (tiles > 0x3fffffffLL) return -1;
   const int most = sm_count() / CG, grid = CG * (tiles < most ? (int)tiles : most);
   cudaLaunchConfig_t cfg = {};
@@ -710,33 +890,93 @@ static int ffn_launch(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cuda
   if (m * ((cols + 127) / 128) >= sm_count()) return ffn_launch_t<128, S, KIND, 1>(g, a, b, st);
   return ffn_launch_t<64, S, KIND, 1>(g, a, b, st);
 }
+
+// How a plain product is cut when its tiles do not fill the machine: slices of k, as many as give every SM (pair) a tile
+// while each keeps at least 512 k.
+struct FfnCut {
+  int splits, pair;      // slices; 256-row tiles of CTA pairs instead of 128-row tiles
+};
+static FfnCut ffn_cut(int M, int m_parts, int N, long long k) {
+  FfnCut c = {1, 0};
+  const int pairs = sm_count() / 2;
+  const long long t2 = (long long)((M + 2 * FF_BM - 1) / (2 * FF_BM)) * m_parts * ((N + 127) / 128);
+  const long long t1 = (long long)((M + FF_BM - 1) / FF_BM) * m_parts * ((N + 63) / 64);
+  if (t2 >= pairs || t1 >= sm_count()) return c;
+  const long long most = k / 512 < 1 ? 1 : k / 512;
+  c.pair = M > FF_BM && t2 * most >= pairs;
+  const long long want = c.pair ? (pairs + t2 - 1) / t2 : (sm_count() + t1 - 1) / t1;
+  c.splits = (int)(want < most ? want : most);
+  if (c.splits < 2) c = {1, 0};
+  return c;
+}
+static long long ffn_plane(int M, int N) { return (long long)((M + 31) / 32 * 32) * ((N + 15) / 16 * 16); }
+// floats of partial sums that a plain product needs
+static long long ffn_cut_floats(int M, int m_parts, int N, long long k) {
+  const FfnCut c = ffn_cut(M, m_parts, N, k);
+  return c.splits > 1 ? c.splits * m_parts * ffn_plane(M, N) : 0;
+}
+
 template <int KIND>
 static int ffn_gemm(int splits, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
   return splits == 3 ? ffn_launch<3, KIND>(g, a, b, st) : ffn_launch<1, KIND>(g, a, b, st);
 }
+// plain product of S operand planes into out [m_parts M, N]; partial: scratch of ffn_cut_floats
+static int ffn_plain(int S, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, void* out, int dt, float* partial, cudaStream_t st) {
+  g.out = out;
+  g.ldo = g.N;
+  g.vec16 = (((uintptr_t)out | (uintptr_t)((long long)g.N * dt_bytes(dt))) & 15) == 0;
+  const long long bk = FF_BK(S);
+  g.k_splits = 1;
+  const FfnCut c = ffn_cut(g.M, g.m_parts, g.N, g.k_blocks * bk * g.segments);
+  if (c.splits == 1) return ffn_gemm<FF_PLAIN>(S, g, a, b, st);
+  if (partial == nullptr) return -1;
+  g.k_splits = c.splits;
+  g.z = partial;
+  g.ldz = (g.N + 15) / 16 * 16;
+  g.z_plane = ffn_plane(g.M, g.N);
+  int rc;
+  if (c.pair) rc = S == 3 ? ffn_launch_t<128, 3, FF_PARTIAL, 2>(g, a, b, st) : ffn_launch_t<128, 1, FF_PARTIAL, 2>(g, a, b, st);
+  else rc = S == 3 ? ffn_launch_t<64, 3, FF_PARTIAL, 1>(g, a, b, st) : ffn_launch_t<64, 1, FF_PARTIAL, 1>(g, a, b, st);
+  if (rc) return rc;
+  const long long runs = g.m_parts * g.z_plane / 8, most = 8LL * sm_count();
+  const dim3 grid((unsigned)((runs + 255) / 256 < most ? (runs + 255) / 256 : most)), block(256);
+  if (dt == DT_F32)
+    return (int)launch_k(ffn_join_kernel<float>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, c.splits, g.m_parts,
+                         g.M, g.N, (float*)out, g.vec16);
+  if (dt == DT_BF16)
+    return (int)launch_k(ffn_join_kernel<__nv_bfloat16>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, c.splits,
+                         g.m_parts, g.M, g.N, (__nv_bfloat16*)out, g.vec16);
+  return (int)launch_k(ffn_join_kernel<__half>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, c.splits, g.m_parts,
+                       g.M, g.N, (__half*)out, g.vec16);
+}
 
-// A matrix the products can read: itself, or its image in the workspace (dst)
-static int ffn_prepare(FfnOperand* o, const void* src, long long rows, int cols, long long ld, int parts, int dt, void* dst,
-                       cudaStream_t st) {
+// A matrix the products can read: itself, or its image `dst` in the workspace, which `images` then has to make (src null:
+// the image is there already)
+static void ffn_prepare(FfnOperand* o, const void* src, long long rows, int cols, long long ld, int parts, int dt, void* dst,
+                        FfnImages* images) {
   o->rows = (int)(rows / parts);
   o->cols = cols;
   o->parts = parts;
   o->splits = dt == DT_F32 ? 3 : 1;
-  if (dst == nullptr) {
-    o->p = src;
-    o->ld = ld;
-    return 0;
+  o->p = dst == nullptr ? src : dst;
+  o->ld = dst == nullptr ? ld : pad16(cols);
+  if (dst == nullptr || src == nullptr) return;
+  FfnImage& m = images->m[images->n++];
+  const uintptr_t bits = (uintptr_t)src | (uintptr_t)(ld * dt_bytes(dt));
+  m.src = src; m.dst = reinterpret_cast<uint16_t*>(dst); m.rows = rows; m.lds = ld; m.cols = cols; m.ldd = pad16(cols);
+  m.vec = bits % (4 * dt_bytes(dt)) == 0 ? 4 : (bits % (2 * dt_bytes(dt)) == 0 ? 2 : 1);
+}
+static int ffn_make_images(FfnImages& images, int dt, cudaStream_t st) {
+  if (images.n == 0) return 0;
+  long long blocks = 0;
+  for (int k = 0; k < images.n; ++k) {
+    images.m[k].first_block = (int)blocks;
+    blocks += (images.m[k].rows + FF_IMG_ROWS - 1) / FF_IMG_ROWS * ((images.m[k].ldd + FF_IMG_SPAN - 1) / FF_IMG_SPAN);
+    if (blocks > 0x7fffffffLL) return -1;
   }
-  o->p = dst;
-  o->ld = pad16(cols);
-  if (src == nullptr) return 0;       // prepared by the forward pass
-  const long long runs = rows * (pad16(cols) / 8);
-  const long long blocks = (runs + 255) / 256, most = 16LL * sm_count();
-  const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(256);
-  const int ldd = pad16(cols);
-  if (dt == DT_F32)
-    return (int)launch_k(ffn_operand_kernel<float, 3>, grid, block, 0, st, (const float*)src, rows, cols, ld, (uint16_t*)dst, ldd);
-  return (int)launch_k(ffn_operand_kernel<uint16_t, 1>, grid, block, 0, st, (const uint16_t*)src, rows, cols, ld, (uint16_t*)dst, ldd);
+  const dim3 grid((unsigned)blocks), block(32 * FF_IMG_ROWS);
+  return (int)(dt == DT_F32 ? launch_k(ffn_operand_kernel<3>, grid, block, 0, st, images)
+                            : launch_k(ffn_operand_kernel<1>, grid, block, 0, st, images));
 }
 
 struct FfnShape {
@@ -747,25 +987,33 @@ static bool ffn_shape_ok(const FfnShape& s) {
   return s.m > 0 && s.d > 0 && s.f > 0 && s.n > 0 && s.dt >= 0 && s.dt <= 2 && s.act >= 0 && s.act <= 3 &&
          s.m < big && s.d < big && 2LL * s.f < big && s.n < big;
 }
-static void ffn_out(FfnGemm& g, void* out, int dt, long long ldo) {
-  g.out = out;
-  g.out_dt = dt;
-  g.ldo = ldo;
-  const uintptr_t bits = (uintptr_t)out | (uintptr_t)(ldo * dt_bytes(dt));
-  g.vec_bytes = bits % 32 == 0 ? 32 : (bits % 16 == 0 ? 16 : 0);
+static long long ffn_kround(long long k, int S) { return (k + FF_BK(S) - 1) / FF_BK(S) * FF_BK(S); }
+
+// floats of the scratch `partial` of either pass (0: none)
+extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt, int backward) {
+  const int S = dt == DT_F32 ? 3 : 1;
+  if (m <= 0 || d <= 0 || f <= 0 || n <= 0) return 0;
+  if (!backward) return ffn_cut_floats(m, 1, n, ffn_kround(f, S));
+  long long a = ffn_cut_floats(m, 1, d, 2 * ffn_kround(f, S));
+  const long long b = ffn_cut_floats(f, 2, d, ffn_kround(m, S)), c = ffn_cut_floats(n, 1, f, ffn_kround(m, S));
+  a = a > b ? a : b;
+  return a > c ? a : c;
 }
 
 // Every operand comes with an optional image: [S][rows][pad16(cols)] 16-bit elements, S = 3 for fp32, needed for fp32 and
-// for rows that do not start on 16-byte boundaries.  h: [S][m][pad16(f)] 16-bit; z: [2][m][pad16(f)] fp32 or null.
+// for rows that do not start on 16-byte boundaries.  h: [S][m][pad16(f)] 16-bit; z: 2 x (m rounded up to 32) x pad16(f) fp32 or null;
+// partial: gated_ffn_partial_floats.
 extern "C" int gated_ffn_forward(const void* x, long long ldx, void* x_img, const void* w_in, long long ld_in, void* in_img,
-                                 const void* w_out, long long ld_out, void* out_img, void* h, float* z, void* y, int m, int d,
-                                 int f, int n, int act, int dt, cudaStream_t st) {
+                                 const void* w_out, long long ld_out, void* out_img, void* h, float* z, float* partial, void* y,
+                                 int m, int d, int f, int n, int act, int dt, cudaStream_t st) {
   const FfnShape s = {m, d, f, n, act, dt};
   if (!ffn_shape_ok(s)) return -1;
   FfnOperand ox, oi, oo;
-  int rc = ffn_prepare(&ox, x, m, d, ldx, 1, dt, x_img, st);
-  if (!rc) rc = ffn_prepare(&oi, w_in, 2LL * f, d, ld_in, 2, dt, in_img, st);
-  if (!rc) rc = ffn_prepare(&oo, w_out, n, f, ld_out, 1, dt, out_img, st);
+  FfnImages images = {};
+  ffn_prepare(&ox, x, m, d, ldx, 1, dt, x_img, &images);
+  ffn_prepare(&oi, w_in, 2LL * f, d, ld_in, 2, dt, in_img, &images);
+  ffn_prepare(&oo, w_out, n, f, ld_out, 1, dt, out_img, &images);
+  int rc = ffn_make_images(images, dt, st);
   if (rc) return rc;
   const int S = dt == DT_F32 ? 3 : 1;
   FfnGemm g = {};
@@ -773,31 +1021,32 @@ extern "C" int gated_ffn_forward(const void* x, long long ldx, void* x_img, cons
   g.act = act;
   g.segments = g.m_parts = g.a_parts = 1;
   g.b_parts = 2;
-  g.M = m; g.N = f; g.k_blocks = (d + FF_BK - 1) / FF_BK;
-  g.out = h; g.ldo = pad16(f); g.z = z; g.ldz = pad16(f);
+  g.M = m; g.N = f; g.k_blocks = (d + FF_BK(S) - 1) / FF_BK(S);
+  g.out = h; g.ldo = pad16(f); g.vec16 = 1; g.z = z; g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
   rc = ffn_gemm<FF_GATE>(S, g, ox, oi, st);
   if (rc) return rc;
   const FfnOperand oh = {h, m, f, 1, S, pad16(f)};
   g.b_parts = 1;
-  g.N = n; g.k_blocks = (f + FF_BK - 1) / FF_BK;
-  ffn_out(g, y, dt, n);
-  return ffn_gemm<FF_PLAIN>(S, g, oh, oo, st);
+  g.N = n; g.k_blocks = (f + FF_BK(S) - 1) / FF_BK(S);
+  return ffn_plain(S, g, oh, oo, y, dt, partial, st);
 }
 
 // x, w_in, w_out: as in the forward pass; where an image is given it holds the forward pass' image already.
 // dz: [S][2][m][pad16(f)] 16-bit scratch.  dx, dw_in, dw_out may be null.
 extern "C" int gated_ffn_backward(const void* x, long long ldx, void* x_img, const void* w_in, long long ld_in, void* in_img,
                                   const void* w_out, long long ld_out, void* out_img, const void* dy, long long ldy,
-                                  void* dy_img, const void* h, const float* z, void* dz, void* dx, void* dw_in, void* dw_out,
+                                  void* dy_img, const void* h, const float* z, void* dz, float* partial, void* dx, void* dw_in, void* dw_out,
                                   int m, int d, int f, int n, int act, int dt, cudaStream_t st) {
   const FfnShape s = {m, d, f, n, act, dt};
   if (!ffn_shape_ok(s)) return -1;
   const int S = dt == DT_F32 ? 3 : 1;
   FfnOperand ox, oi, oo, oy;
-  int rc = ffn_prepare(&oy, dy, m, n, ldy, 1, dt, dy_img, st);
-  if (!rc) rc = ffn_prepare(&ox, x_img != nullptr ? nullptr : x, m, d, ldx, 1, dt, x_img, st);
-  if (!rc) rc = ffn_prepare(&oi, in_img != nullptr ? nullptr : w_in, 2LL * f, d, ld_in, 2, dt, in_img, st);
-  if (!rc) rc = ffn_prepare(&oo, out_img != nullptr ? nullptr : w_out, n, f, ld_out, 1, dt, out_img, st);
+  FfnImages images = {};
+  ffn_prepare(&oy, dy, m, n, ldy, 1, dt, dy_img, &images);
+  ffn_prepare(&ox, x_img != nullptr ? nullptr : x, m, d, ldx, 1, dt, x_img, &images);
+  ffn_prepare(&oi, in_img != nullptr ? nullptr : w_in, 2LL * f, d, ld_in, 2, dt, in_img, &images);
+  ffn_prepare(&oo, out_img != nullptr ? nullptr : w_out, n, f, ld_out, 1, dt, out_img, &images);
+  int rc = ffn_make_images(images, dt, st);
   if (rc) return rc;
   const FfnOperand oh = {h, m, f, 1, S, pad16(f)}, oz = {dz, m, f, 2, S, pad16(f)};
   FfnGemm base = {};
@@ -806,27 +1055,24 @@ extern "C" int gated_ffn_backward(const void* x, long long ldx, void* x_img, con
   base.segments = base.m_parts = base.a_parts = base.b_parts = 1;
   FfnGemm g = base;
   if (dx != nullptr || dw_in != nullptr) {
-    g.M = m; g.N = f; g.k_blocks = (n + FF_BK - 1) / FF_BK; g.b_mn = 1;
-    g.out = dz; g.ldo = pad16(f); g.z = const_cast<float*>(z); g.ldz = pad16(f);
+    g.M = m; g.N = f; g.k_blocks = (n + FF_BK(S) - 1) / FF_BK(S); g.b_mn = 1;
+    g.out = dz; g.ldo = pad16(f); g.vec16 = 1; g.z = const_cast<float*>(z); g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
     if ((rc = ffn_gemm<FF_DGATE>(S, g, oy, oo, st))) return rc;
   }
   if (dx != nullptr) {
     g = base;
-    g.M = m; g.N = d; g.k_blocks = (f + FF_BK - 1) / FF_BK; g.segments = 2; g.a_parts = g.b_parts = 2; g.b_mn = 1;
-    ffn_out(g, dx, dt, d);
-    if ((rc = ffn_gemm<FF_PLAIN>(S, g, oz, oi, st))) return rc;
+    g.M = m; g.N = d; g.k_blocks = (f + FF_BK(S) - 1) / FF_BK(S); g.segments = 2; g.a_parts = g.b_parts = 2; g.b_mn = 1;
+    if ((rc = ffn_plain(S, g, oz, oi, dx, dt, partial, st))) return rc;
   }
   if (dw_in != nullptr) {
     g = base;
-    g.M = f; g.N = d; g.k_blocks = (m + FF_BK - 1) / FF_BK; g.m_parts = g.a_parts = 2; g.a_mn = g.b_mn = 1;
-    ffn_out(g, dw_in, dt, d);
-    if ((rc = ffn_gemm<FF_PLAIN>(S, g, oz, ox, st))) return rc;
+    g.M = f; g.N = d; g.k_blocks = (m + FF_BK(S) - 1) / FF_BK(S); g.m_parts = g.a_parts = 2; g.a_mn = g.b_mn = 1;
+    if ((rc = ffn_plain(S, g, oz, ox, dw_in, dt, partial, st))) return rc;
   }
   if (dw_out != nullptr) {
     g = base;
-    g.M = n; g.N = f; g.k_blocks = (m + FF_BK - 1) / FF_BK; g.a_mn = g.b_mn = 1;
-    ffn_out(g, dw_out, dt, f);
-    if ((rc = ffn_gemm<FF_PLAIN>(S, g, oy, oh, st))) return rc;
+    g.M = n; g.N = f; g.k_blocks = (m + FF_BK(S) - 1) / FF_BK(S); g.a_mn = g.b_mn = 1;
+    if ((rc = ffn_plain(S, g, oy, oh, dw_out, dt, partial, st))) return rc;
   }
   return 0;
 }

@@ -21,9 +21,11 @@ def _declare():
     lib = _lib.load()
     if not getattr(lib, "_ffn_declared", False):
         vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        lib.gated_ffn_forward.argtypes = [vp, ll, vp] * 3 + [vp] * 3 + [i] * 6 + [vp]
-        lib.gated_ffn_backward.argtypes = [vp, ll, vp] * 4 + [vp] * 6 + [i] * 6 + [vp]
+        lib.gated_ffn_forward.argtypes = [vp, ll, vp] * 3 + [vp] * 4 + [i] * 6 + [vp]
+        lib.gated_ffn_backward.argtypes = [vp, ll, vp] * 4 + [vp] * 7 + [i] * 6 + [vp]
         lib.gated_ffn_forward.restype = lib.gated_ffn_backward.restype = lib.gated_ffn_last_error.restype = i
+        lib.gated_ffn_partial_floats.argtypes = [i] * 6
+        lib.gated_ffn_partial_floats.restype = ll
         lib._ffn_declared = True
     return lib
 
@@ -35,6 +37,10 @@ def last_error() -> int:
 
 def _pad16(n: int) -> int:
     return (n + 15) // 16 * 16
+
+
+def _pad32(n: int) -> int:
+    return (n + 31) // 32 * 32
 
 
 def _aligned(t: torch.Tensor) -> bool:
@@ -51,6 +57,9 @@ class _Layout:
         at = self.size
         self.size += (nbytes + 255) // 256 * 256
         return at
+
+    def scratch(self, floats: int):
+        return self.add(4 * floats) if floats else None
 
     def image(self, t: torch.Tensor):
         """Room for the operand image of a matrix, or None where it is read as it is."""
@@ -75,13 +84,14 @@ class _GatedFfnFn(torch.autograd.Function):
         img = [lay.image(t) for t in (x2, wi, wo)]
         planes = 3 if x.dtype == torch.float32 else 1
         h = lay.add(planes * m * _pad16(f) * 2)
-        z = lay.add(2 * m * _pad16(f) * 4) if train else None
+        z = lay.add(2 * _pad32(m) * _pad16(f) * 4) if train else None
+        partial = lay.scratch(lib.gated_ffn_partial_floats(m, d, f, n, DT[x.dtype], 0))
         buf = torch.empty(lay.size, dtype=torch.uint8, device=x.device)
         if m:
             b = buf.data_ptr()
             rc = lib.gated_ffn_forward(x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
-                                       wo.data_ptr(), wo.stride(0), _at(b, img[2]), b + h, _at(b, z), y.data_ptr(), m, d, f, n,
-                                       act, DT[x.dtype], _lib.stream_ptr())
+                                       wo.data_ptr(), wo.stride(0), _at(b, img[2]), b + h, _at(b, z), _at(b, partial), y.data_ptr(), m, d, f,
+                                       n, act, DT[x.dtype], _lib.stream_ptr())
             if rc:
                 raise RuntimeError(f"gated_ffn_forward failed with code {rc}")
             _lib.count(2 + sum(i is not None for i in img))
@@ -107,12 +117,13 @@ class _GatedFfnFn(torch.autograd.Function):
             lay = _Layout()
             dy_img = lay.image(dy2)
             dz = lay.add((3 if x2.dtype == torch.float32 else 1) * 2 * m * _pad16(f) * 2)
+            partial = lay.scratch(lib.gated_ffn_partial_floats(m, d, f, n, DT[x2.dtype], 1))
             scratch = torch.empty(lay.size, dtype=torch.uint8, device=x2.device)
             b, s = buf.data_ptr(), scratch.data_ptr()
             rc = lib.gated_ffn_backward(x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
                                         wo.data_ptr(), wo.stride(0), _at(b, img[2]), dy2.data_ptr(), dy2.stride(0),
-                                        _at(s, dy_img), b + h, b + z, s + dz, _lib.ptr(dx), _lib.ptr(dwi), _lib.ptr(dwo), m, d,
-                                        f, n, ctx.act, DT[x2.dtype], _lib.stream_ptr())
+                                        _at(s, dy_img), b + h, b + z, s + dz, _at(s, partial), _lib.ptr(dx), _lib.ptr(dwi),
+                                        _lib.ptr(dwo), m, d, f, n, ctx.act, DT[x2.dtype], _lib.stream_ptr())
             if rc:
                 raise RuntimeError(f"gated_ffn_backward failed with code {rc}")
             _lib.count(int(need[0] or need[1]) + sum(need[:3]) + int(dy_img is not None))
