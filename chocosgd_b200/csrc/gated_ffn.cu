@@ -209,7 +209,7 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t (&q)[3]) {
   }
 }
 
-// activation and (wanted) its derivative.  The quotient is the approximate one (2 units of the last place); FAST: so is the
+// activation and (wanted) its derivative.  The reciprocal is the approximate one (1 unit of the last place); FAST: so is the
 // exponential (relative error |z| 2^-23), which suits 16-bit results.
 template <int ACT, bool GRAD, bool FAST>
 __device__ __forceinline__ float ff_act(float z, float& slope) {
@@ -225,13 +225,14 @@ __device__ __forceinline__ float ff_act(float z, float& slope) {
     if (GRAD) slope = z > 0.f ? 1.f : 0.f;
     return z < 0.f ? 0.f : z;
   }
-  // __fdividef gives 0 for divisors above 2^126, which is the limit wanted here
-  const float sg = __fdividef(1.f, 1.f + (FAST ? __expf(-z) : expf(-z)));
+  float sg;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(sg) : "f"(1.f + (FAST ? __expf(-z) : expf(-z))));
   if (ACT == ACT_SILU) {
-    if (GRAD) slope = sg * fmaf(z, 1.f - sg, 1.f);
-    return z * sg;
+    const float a = z * sg;
+    if (GRAD) slope = fmaf(a, 1.f - sg, sg);
+    return a;
   }
-  if (GRAD) slope = sg * (1.f - sg);
+  if (GRAD) slope = fmaf(-sg, sg, sg);
   return sg;
 }
 
@@ -291,6 +292,7 @@ template <int S, int KIND, int HC, int ACT> struct FfnEpilogue {
   const FfnGemm& g;
   uint8_t* stage;
   int m_part, row0, col0, lane;      // first row and column of the warp
+  float* z;                          // this lane's place of (row0, col0) in z; 16 columns are 512 floats
 
   __device__ __forceinline__ void put(int c, const float* v, const float* u, const float* zg, const float* zu) {
     constexpr bool FAST = S == 1;
@@ -298,11 +300,11 @@ template <int S, int KIND, int HC, int ACT> struct FfnEpilogue {
     if (KIND == FF_GATE) {
       float h[16], slope;
       if (g.z != nullptr && row0 < g.M && col < g.N) {
-        float* z = g.z + lane_off(row0 + lane, col, g.ldz);
+        float *zg_at = z + c * 32, *zu_at = zg_at + g.z_plane;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          st32b(z + k * 256, reinterpret_cast<const uint32_t*>(v + 8 * k));
-          st32b(z + k * 256 + g.z_plane, reinterpret_cast<const uint32_t*>(u + 8 * k));
+          st32b(zg_at + k * 256, reinterpret_cast<const uint32_t*>(v + 8 * k));
+          st32b(zu_at + k * 256, reinterpret_cast<const uint32_t*>(u + 8 * k));
         }
       }
 #pragma unroll
@@ -322,9 +324,8 @@ template <int S, int KIND, int HC, int ACT> struct FfnEpilogue {
       operand<(HC < 32 ? HC : 32)>(c, 4, du, plane, 2 * plane);
     } else if (KIND == FF_PARTIAL) {
       if (row0 < g.M && col < g.N) {
-        float* z = g.z + m_part * g.z_plane + lane_off(row0 + lane, col, g.ldz);
-        st32b(z, reinterpret_cast<const uint32_t*>(v));
-        st32b(z + 256, reinterpret_cast<const uint32_t*>(v + 8));
+        st32b(z + c * 32, reinterpret_cast<const uint32_t*>(v));
+        st32b(z + c * 32 + 256, reinterpret_cast<const uint32_t*>(v + 8));
       }
     } else if (S == 3) {
       constexpr int FC = HC < 32 ? HC : 32;
@@ -374,14 +375,13 @@ template <int S, int KIND, int HC, int ACT> struct FfnEpilogue {
     }
   }
 };
-// G and U of sixteen columns of a row (dgate); zeros outside
-__device__ __forceinline__ void ff_load_z(const FfnGemm& g, int row0, int lane, int col, float* zg, float* zu) {
-  if (row0 < g.M && col < g.N) {
-    const float* z = g.z + lane_off(row0 + lane, col, g.ldz);
+// G and U of sixteen columns of a row (dgate) from this lane's place in z; zeros outside
+__device__ __forceinline__ void ff_load_z(const float* z, long long z_plane, bool inside, float* zg, float* zu) {
+  if (inside) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       ld32b(z + k * 256, reinterpret_cast<uint32_t*>(zg + 8 * k));
-      ld32b(z + k * 256 + g.z_plane, reinterpret_cast<uint32_t*>(zu + 8 * k));
+      ld32b(z + z_plane + k * 256, reinterpret_cast<uint32_t*>(zu + 8 * k));
     }
   } else {
 #pragma unroll
@@ -608,6 +608,9 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
       const int m_part = tm / tiles_m;
       const int z_index = KIND == FF_PARTIAL ? tile / out_tiles * g.m_parts + m_part : m_part;
       const int row0 = (tm % tiles_m) * TM + (int)rank * FF_BM + (warp & 3) * 32, col0 = tn * BN_OUT + half * HC;
+      float* z = KIND == FF_PLAIN || g.z == nullptr
+                     ? nullptr : g.z + (KIND == FF_PARTIAL ? z_index * g.z_plane : 0) + lane_off(row0 + lane, col0, g.ldz);
+      const int z_cols = row0 < g.M ? g.N - col0 : 0;      // columns of z that exist
       bool stop = false;
       if (S == 3) {
         // the accumulators of every 64 k, added up in registers
@@ -643,11 +646,11 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
         }
         if (!stop) {
           ff_for_act<KIND>(g.act, [&](auto act) {
-            FfnEpilogue<S, KIND, HC, decltype(act)::value> epi = {g, epi_smem + warp * 4096, z_index, row0, col0, lane};
+            FfnEpilogue<S, KIND, HC, decltype(act)::value> epi = {g, epi_smem + warp * 4096, m_part, row0, col0, lane, z};
             float zg[16], zu[16];
 #pragma unroll
             for (int c = 0; c < HC; c += 16) {
-              if (KIND == FF_DGATE) ff_load_z(g, row0, lane, col0 + c, zg, zu);
+              if (KIND == FF_DGATE) ff_load_z(z + c * 32, g.z_plane, c < z_cols, zg, zu);
               epi.put(c, acc + c, acc + (KIND == FF_GATE ? HC + c : c), zg, zu);
             }
           });
@@ -657,25 +660,25 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
         // dgate: G and U of the next sixteen columns are under way while the present ones are worked on; the first ones
         // while the tile is still being multiplied
         float zg[16], zu[16], yg[16], yu[16];
-        if (KIND == FF_DGATE) ff_load_z(g, row0, lane, col0, zg, zu);
+        if (KIND == FF_DGATE) ff_load_z(z, g.z_plane, 0 < z_cols, zg, zu);
         const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
         if (ff_epi_bar_or(bad)) stop = true;
         else {
           tc_fence_after();
           ff_for_act<KIND>(g.act, [&](auto act) {
-            FfnEpilogue<S, KIND, HC, decltype(act)::value> epi = {g, epi_smem + warp * 4096, z_index, row0, col0, lane};
+            FfnEpilogue<S, KIND, HC, decltype(act)::value> epi = {g, epi_smem + warp * 4096, m_part, row0, col0, lane, z};
             const uint32_t acc = tmem_base + lanes + buf * BN + half * HC;
 #pragma unroll 1
             for (int c = 0; c < HC; c += 32) {
               float v[16], u[16];
-              if (KIND == FF_DGATE && c + 16 < HC) ff_load_z(g, row0, lane, col0 + c + 16, yg, yu);
+              if (KIND == FF_DGATE && c + 16 < HC) ff_load_z(z + c * 32 + 512, g.z_plane, c + 16 < z_cols, yg, yu);
               tmem_ld16_async(acc + c, v);
               if (KIND == FF_GATE) tmem_ld16_async(acc + BN_OUT + c, u);
               tmem_wait16(v);
               if (KIND == FF_GATE) tmem_wait16(u);
               epi.put(c, v, u, zg, zu);
               if (HC < 32) break;
-              if (KIND == FF_DGATE && c + 32 < HC) ff_load_z(g, row0, lane, col0 + c + 32, zg, zu);
+              if (KIND == FF_DGATE && c + 32 < HC) ff_load_z(z + c * 32 + 1024, g.z_plane, c + 32 < z_cols, zg, zu);
               tmem_ld16_async(acc + c + 16, v);
               if (KIND == FF_GATE) tmem_ld16_async(acc + BN_OUT + c + 16, u);
               tmem_wait16(v);
@@ -713,26 +716,23 @@ struct FfnImage {
   uint16_t* dst;
   long long rows, lds;
   int cols, ldd, vec;       // vec: elements per access that the row starts allow (1, 2, 4)
-  int first_block;          // blocks [first_block, next image's) copy this matrix
+  unsigned first_block;     // blocks [first_block, next image's) copy this matrix, eight elements per thread
 };
 struct FfnImages {
   FfnImage m[3];
   int n;
 };
-#define FF_IMG_ROWS 8       // rows per block, one per warp
-#define FF_IMG_SPAN 4096    // columns per block
 template <int S>
-__global__ void __launch_bounds__(32 * FF_IMG_ROWS) ffn_operand_kernel(const __grid_constant__ FfnImages a) {
+__global__ void __launch_bounds__(256) ffn_operand_kernel(const __grid_constant__ FfnImages a) {
   pdl_wait();
   pdl_trigger();
   int k = 0;
-  while (k + 1 < a.n && (int)blockIdx.x >= a.m[k + 1].first_block) ++k;
+  while (k + 1 < a.n && blockIdx.x >= a.m[k + 1].first_block) ++k;
   const FfnImage& m = a.m[k];
-  const int spans = (m.ldd + FF_IMG_SPAN - 1) / FF_IMG_SPAN, b = (int)blockIdx.x - m.first_block;
-  const long long r = (long long)(b / spans) * FF_IMG_ROWS + (threadIdx.x >> 5);
-  if (r >= m.rows) return;
-  const int c_end = min(m.ldd, (b % spans + 1) * FF_IMG_SPAN);
-  for (int c = (b % spans) * FF_IMG_SPAN + (threadIdx.x & 31) * 8; c < c_end; c += 256) {
+  const unsigned per_row = m.ldd / 8, i = (blockIdx.x - m.first_block) * 256 + threadIdx.x;
+  const long long r = i / per_row;
+  const int c = (int)(i - (unsigned)r * per_row) * 8;
+  if (r < m.rows) {
     uint16_t* q = m.dst + r * m.ldd + c;
     if (S == 3) {
       const float* p = reinterpret_cast<const float*>(m.src) + r * m.lds + c;
@@ -777,40 +777,34 @@ __global__ void __launch_bounds__(32 * FF_IMG_ROWS) ffn_operand_kernel(const __g
   }
 }
 
-// out [m_parts M, N] = sum over k_splits slices of partial sums, in slice order; one thread per 8 columns
+// out [m_parts M, N] = sum over k_splits slices of partial sums, in slice order.  A block takes 32 rows x 64 columns: eight
+// warps read eight lane-blocked groups each slice, and rows are written as they lie in memory.
 template <typename T>
 __global__ void __launch_bounds__(256) ffn_join_kernel(const float* z, long long ldz, long long z_plane, int splits, int m_parts,
-                                                       int M, int N, T* out, int vec16) {
+                                                       int M, int N, T* out) {
+  __shared__ float tile[32][65];
   pdl_wait();
   pdl_trigger();
-  const int groups = (int)(ldz >> 3), blocks = (M + 31) / 32, lane = threadIdx.x & 31;
-  const int total = m_parts * blocks * groups;      // one warp each
-  for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < total; j += gridDim.x * 8) {
-    const int rb = j / groups, col = (j - rb * groups) * 8, part = rb / blocks, row = (rb - part * blocks) * 32 + lane;
-    if (row >= M || col >= N) continue;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = (M + 31) / 32;
+  const int part = blockIdx.y / blocks, row0 = (blockIdx.y - part * blocks) * 32, col0 = blockIdx.x * 64;
+  if (col0 + warp * 8 < ldz) {
     float v[8], w[8];
-    const float* p = z + part * z_plane + lane_off(row, col, ldz);
+    const float* p = z + part * z_plane + lane_off(row0 + lane, col0 + warp * 8, ldz);
     ld32b(p, reinterpret_cast<uint32_t*>(v));
+#pragma unroll 4
     for (int q = 1; q < splits; ++q) {
       ld32b(p + (long long)q * m_parts * z_plane, reinterpret_cast<uint32_t*>(w));
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
-    T* o = out + ((long long)part * M + row) * N + col;
-    constexpr int W = 16 / (int)sizeof(T);
-    if (vec16 && col + 8 <= N) {
 #pragma unroll
-      for (int h = 0; h < 8; h += W) {
-        Vec<T, W> r;
+    for (int e = 0; e < 8; ++e) tile[lane][warp * 8 + e] = v[e];
+  }
+  __syncthreads();
 #pragma unroll
-        for (int e = 0; e < W; ++e) r.e[e] = from_f<T>(v[(h + e) & 7]);
-        r.store(o + h);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (col + e < N) o[e] = from_f<T>(v[e]);
-    }
+  for (int k = 0; k < 8; ++k) {
+    const int i = k * 256 + threadIdx.x, r = i >> 6, c = i & 63;
+    if (row0 + r < M && col0 + c < N) out[((long long)part * M + row0 + r) * N + col0 + c] = from_f<T>(tile[r][c]);
   }
 }
 
@@ -878,76 +872,91 @@ static int ffn_launch_t(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cu
   return (int)cudaLaunchKernelEx(&cfg, kernel, g);
 }
 
-// Tile by the number of tiles: the widest that still gives every SM (pair) one (a narrow tile reads more operand bytes per
-// multiplication; an idle SM costs more).
-template <int S, int KIND>
-static int ffn_launch(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
-  const int cols = KIND == FF_GATE ? 2 * g.N : g.N, pairs = sm_count() / 2;
-  const long long m2 = (long long)((g.M + 2 * FF_BM - 1) / (2 * FF_BM)) * g.m_parts;
-  if (m2 * ((cols + 255) / 256) >= pairs) return ffn_launch_t<256, S, KIND, 2>(g, a, b, st);
-  if (m2 * ((cols + 127) / 128) >= pairs) return ffn_launch_t<128, S, KIND, 2>(g, a, b, st);
-  const long long m = (long long)((g.M + FF_BM - 1) / FF_BM) * g.m_parts;
-  if (m * ((cols + 127) / 128) >= sm_count()) return ffn_launch_t<128, S, KIND, 1>(g, a, b, st);
-  return ffn_launch_t<64, S, KIND, 1>(g, a, b, st);
-}
-
-// How a plain product is cut when its tiles do not fill the machine: slices of k, as many as give every SM (pair) a tile
-// while each keeps at least 512 k.
-struct FfnCut {
-  int splits, pair;      // slices; 256-row tiles of CTA pairs instead of 128-row tiles
+// Which tile a product runs with, by its time in SM cycles:  rounds x (64-k blocks x step + exposed epilogue), where
+//   rounds    tiles per SM (pair), rounded up
+//   step      the slower of multiplying (1024 multiply-adds x 4 per cycle and SM; six times for three planes) and of fetching
+//             the operands (measured: about 58 bytes per cycle and SM from L2 when all SMs fetch)
+//   epilogue  runs under the next tile's multiplications for 16-bit operands, not for three planes (whose sums are in the
+//             epilogue's registers)
+// and, for a plain product cut into slices of k, the partial sums' second pass (a launch, then 4 bytes of each written and read).
+struct FfnTile {
+  int bn, cg, splits;
 };
-static FfnCut ffn_cut(int M, int m_parts, int N, long long k) {
-  FfnCut c = {1, 0};
-  const int pairs = sm_count() / 2;
-  const long long t2 = (long long)((M + 2 * FF_BM - 1) / (2 * FF_BM)) * m_parts * ((N + 127) / 128);
-  const long long t1 = (long long)((M + FF_BM - 1) / FF_BM) * m_parts * ((N + 63) / 64);
-  if (t2 >= pairs || t1 >= sm_count()) return c;
-  const long long most = k / 512 < 1 ? 1 : k / 512;
-  c.pair = M > FF_BM && t2 * most >= pairs;
-  const long long want = c.pair ? (pairs + t2 - 1) / t2 : (sm_count() + t1 - 1) / t1;
-  c.splits = (int)(want < most ? want : most);
-  if (c.splits < 2) c = {1, 0};
+static double ffn_cost(const FfnTile& t, int S, int kind, int M, int m_parts, int cols, long long k64) {
+  const int sms = sm_count() / t.cg, tm = FF_BM * t.cg;
+  const double tiles = (double)((M + tm - 1) / tm) * m_parts * ((cols + t.bn - 1) / t.bn) * t.splits;
+  const double rounds = (double)(long long)((tiles + sms - 1) / sms);
+  const double mul = 2.0 * t.bn * (S == 3 ? 6 : 1), fetch = S * (FF_BM + t.bn / t.cg) * 128.0 / 58.0;
+  const double step = mul > fetch ? mul : fetch, main = (double)((k64 + t.splits - 1) / t.splits) * step;
+  const double epi = t.bn * (kind == FF_DGATE ? 70.0 : 45.0);
+  double c = S == 3 ? rounds * (main + epi) : rounds * (main > epi ? main : epi) + epi;
+  c += 3000.0;                                               // launch, first loads
+  if (t.splits > 1) c += 5000.0 + 8.0 * t.splits * m_parts * M * cols / (30.0 * sm_count());
   return c;
 }
+// the cheapest of: pairs 256 / 128 wide, single CTAs 128 / 64 wide; a plain product also in up to 16 slices of at least 256 k
+// (not 256 wide: there the tiles are many)
+static FfnTile ffn_tile_for(int S, int kind, int M, int m_parts, int cols, long long k64) {
+  static const FfnTile shapes[4] = {{256, 2, 1}, {128, 2, 1}, {128, 1, 1}, {64, 1, 1}};
+  FfnTile best = shapes[0];
+  double cost = 1e300;
+  for (int i = 0; i < 4; ++i) {
+    if (shapes[i].cg == 2 && M <= FF_BM) continue;
+    for (int q = 1; q <= (kind == FF_PLAIN && (i == 1 || i == 3) ? 16 : 1); ++q) {
+      if (q > 1 && (k64 / q < 4 || (long long)m_parts * ((M + 31) / 32) > 65535)) break;    // 65535: grid of ffn_join_kernel
+      FfnTile t = shapes[i];
+      t.splits = q;
+      const double c = ffn_cost(t, S, kind, M, m_parts, cols, k64);
+      if (c < cost) { cost = c; best = t; }
+    }
+  }
+  return best;
+}
+template <int S, int KIND>
+static int ffn_launch(const FfnTile& t, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
+  if (t.cg == 2) return t.bn == 256 ? ffn_launch_t<256, S, KIND, 2>(g, a, b, st) : ffn_launch_t<128, S, KIND, 2>(g, a, b, st);
+  return t.bn == 128 ? ffn_launch_t<128, S, KIND, 1>(g, a, b, st) : ffn_launch_t<64, S, KIND, 1>(g, a, b, st);
+}
+
 static long long ffn_plane(int M, int N) { return (long long)((M + 31) / 32 * 32) * ((N + 15) / 16 * 16); }
+static long long ffn_k64(int S, int k_blocks, int segments) { return ((long long)k_blocks * segments * FF_BK(S) + 63) / 64; }
+static int ffn_k_blocks(int S, int k) { return (k + FF_BK(S) - 1) / FF_BK(S); }
 // floats of partial sums that a plain product needs
-static long long ffn_cut_floats(int M, int m_parts, int N, long long k) {
-  const FfnCut c = ffn_cut(M, m_parts, N, k);
-  return c.splits > 1 ? c.splits * m_parts * ffn_plane(M, N) : 0;
+static long long ffn_partial_floats(int S, int M, int m_parts, int N, int k, int segments) {
+  const FfnTile t = ffn_tile_for(S, FF_PLAIN, M, m_parts, N, ffn_k64(S, ffn_k_blocks(S, k), segments));
+  return t.splits > 1 ? t.splits * m_parts * ffn_plane(M, N) : 0;
 }
 
 template <int KIND>
-static int ffn_gemm(int splits, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
-  return splits == 3 ? ffn_launch<3, KIND>(g, a, b, st) : ffn_launch<1, KIND>(g, a, b, st);
+static int ffn_gemm(int S, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
+  const FfnTile t = ffn_tile_for(S, KIND, g.M, g.m_parts, KIND == FF_GATE ? 2 * g.N : g.N, ffn_k64(S, g.k_blocks, g.segments));
+  return S == 3 ? ffn_launch<3, KIND>(t, g, a, b, st) : ffn_launch<1, KIND>(t, g, a, b, st);
 }
-// plain product of S operand planes into out [m_parts M, N]; partial: scratch of ffn_cut_floats
+// plain product of S operand planes into out [m_parts M, N]; partial: scratch of ffn_partial_floats
 static int ffn_plain(int S, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, void* out, int dt, float* partial, cudaStream_t st) {
   g.out = out;
   g.ldo = g.N;
   g.vec16 = (((uintptr_t)out | (uintptr_t)((long long)g.N * dt_bytes(dt))) & 15) == 0;
-  const long long bk = FF_BK(S);
-  g.k_splits = 1;
-  const FfnCut c = ffn_cut(g.M, g.m_parts, g.N, g.k_blocks * bk * g.segments);
-  if (c.splits == 1) return ffn_gemm<FF_PLAIN>(S, g, a, b, st);
+  const FfnTile t = ffn_tile_for(S, FF_PLAIN, g.M, g.m_parts, g.N, ffn_k64(S, g.k_blocks, g.segments));
+  g.k_splits = t.splits;
+  if (t.splits == 1) return S == 3 ? ffn_launch<3, FF_PLAIN>(t, g, a, b, st) : ffn_launch<1, FF_PLAIN>(t, g, a, b, st);
   if (partial == nullptr) return -1;
-  g.k_splits = c.splits;
   g.z = partial;
   g.ldz = (g.N + 15) / 16 * 16;
   g.z_plane = ffn_plane(g.M, g.N);
   int rc;
-  if (c.pair) rc = S == 3 ? ffn_launch_t<128, 3, FF_PARTIAL, 2>(g, a, b, st) : ffn_launch_t<128, 1, FF_PARTIAL, 2>(g, a, b, st);
+  if (t.cg == 2) rc = S == 3 ? ffn_launch_t<128, 3, FF_PARTIAL, 2>(g, a, b, st) : ffn_launch_t<128, 1, FF_PARTIAL, 2>(g, a, b, st);
   else rc = S == 3 ? ffn_launch_t<64, 3, FF_PARTIAL, 1>(g, a, b, st) : ffn_launch_t<64, 1, FF_PARTIAL, 1>(g, a, b, st);
   if (rc) return rc;
-  const long long runs = g.m_parts * g.z_plane / 8, most = 8LL * sm_count();
-  const dim3 grid((unsigned)((runs + 255) / 256 < most ? (runs + 255) / 256 : most)), block(256);
+  const dim3 grid((g.N + 63) / 64, g.m_parts * ((g.M + 31) / 32)), block(256);
   if (dt == DT_F32)
-    return (int)launch_k(ffn_join_kernel<float>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, c.splits, g.m_parts,
-                         g.M, g.N, (float*)out, g.vec16);
+    return (int)launch_k(ffn_join_kernel<float>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, g.k_splits, g.m_parts,
+                         g.M, g.N, (float*)out);
   if (dt == DT_BF16)
-    return (int)launch_k(ffn_join_kernel<__nv_bfloat16>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, c.splits,
-                         g.m_parts, g.M, g.N, (__nv_bfloat16*)out, g.vec16);
-  return (int)launch_k(ffn_join_kernel<__half>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, c.splits, g.m_parts,
-                       g.M, g.N, (__half*)out, g.vec16);
+    return (int)launch_k(ffn_join_kernel<__nv_bfloat16>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, g.k_splits,
+                         g.m_parts, g.M, g.N, (__nv_bfloat16*)out);
+  return (int)launch_k(ffn_join_kernel<__half>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, g.k_splits, g.m_parts,
+                       g.M, g.N, (__half*)out);
 }
 
 // A matrix the products can read: itself, or its image `dst` in the workspace, which `images` then has to make (src null:
@@ -970,11 +979,12 @@ static int ffn_make_images(FfnImages& images, int dt, cudaStream_t st) {
   if (images.n == 0) return 0;
   long long blocks = 0;
   for (int k = 0; k < images.n; ++k) {
-    images.m[k].first_block = (int)blocks;
-    blocks += (images.m[k].rows + FF_IMG_ROWS - 1) / FF_IMG_ROWS * ((images.m[k].ldd + FF_IMG_SPAN - 1) / FF_IMG_SPAN);
-    if (blocks > 0x7fffffffLL) return -1;
+    const long long runs = images.m[k].rows * (images.m[k].ldd / 8);
+    images.m[k].first_block = (unsigned)blocks;
+    blocks += (runs + 255) / 256;
+    if (runs > 0xffffff00LL || blocks > 0x7fffffffLL) return -1;
   }
-  const dim3 grid((unsigned)blocks), block(32 * FF_IMG_ROWS);
+  const dim3 grid((unsigned)blocks), block(256);
   return (int)(dt == DT_F32 ? launch_k(ffn_operand_kernel<3>, grid, block, 0, st, images)
                             : launch_k(ffn_operand_kernel<1>, grid, block, 0, st, images));
 }
@@ -987,15 +997,13 @@ static bool ffn_shape_ok(const FfnShape& s) {
   return s.m > 0 && s.d > 0 && s.f > 0 && s.n > 0 && s.dt >= 0 && s.dt <= 2 && s.act >= 0 && s.act <= 3 &&
          s.m < big && s.d < big && 2LL * s.f < big && s.n < big;
 }
-static long long ffn_kround(long long k, int S) { return (k + FF_BK(S) - 1) / FF_BK(S) * FF_BK(S); }
-
 // floats of the scratch `partial` of either pass (0: none)
 extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt, int backward) {
   const int S = dt == DT_F32 ? 3 : 1;
   if (m <= 0 || d <= 0 || f <= 0 || n <= 0) return 0;
-  if (!backward) return ffn_cut_floats(m, 1, n, ffn_kround(f, S));
-  long long a = ffn_cut_floats(m, 1, d, 2 * ffn_kround(f, S));
-  const long long b = ffn_cut_floats(f, 2, d, ffn_kround(m, S)), c = ffn_cut_floats(n, 1, f, ffn_kround(m, S));
+  if (!backward) return ffn_partial_floats(S, m, 1, n, f, 1);
+  long long a = ffn_partial_floats(S, m, 1, d, f, 2);
+  const long long b = ffn_partial_floats(S, f, 2, d, m, 1), c = ffn_partial_floats(S, n, 1, f, m, 1);
   a = a > b ? a : b;
   return a > c ? a : c;
 }
@@ -1021,13 +1029,13 @@ extern "C" int gated_ffn_forward(const void* x, long long ldx, void* x_img, cons
   g.act = act;
   g.segments = g.m_parts = g.a_parts = 1;
   g.b_parts = 2;
-  g.M = m; g.N = f; g.k_blocks = (d + FF_BK(S) - 1) / FF_BK(S);
+  g.M = m; g.N = f; g.k_blocks = ffn_k_blocks(S, d);
   g.out = h; g.ldo = pad16(f); g.vec16 = 1; g.z = z; g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
   rc = ffn_gemm<FF_GATE>(S, g, ox, oi, st);
   if (rc) return rc;
   const FfnOperand oh = {h, m, f, 1, S, pad16(f)};
   g.b_parts = 1;
-  g.N = n; g.k_blocks = (f + FF_BK(S) - 1) / FF_BK(S);
+  g.N = n; g.k_blocks = ffn_k_blocks(S, f);
   return ffn_plain(S, g, oh, oo, y, dt, partial, st);
 }
 
@@ -1055,23 +1063,23 @@ extern "C" int gated_ffn_backward(const void* x, long long ldx, void* x_img, con
   base.segments = base.m_parts = base.a_parts = base.b_parts = 1;
   FfnGemm g = base;
   if (dx != nullptr || dw_in != nullptr) {
-    g.M = m; g.N = f; g.k_blocks = (n + FF_BK(S) - 1) / FF_BK(S); g.b_mn = 1;
+    g.M = m; g.N = f; g.k_blocks = ffn_k_blocks(S, n); g.b_mn = 1;
     g.out = dz; g.ldo = pad16(f); g.vec16 = 1; g.z = const_cast<float*>(z); g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
     if ((rc = ffn_gemm<FF_DGATE>(S, g, oy, oo, st))) return rc;
   }
   if (dx != nullptr) {
     g = base;
-    g.M = m; g.N = d; g.k_blocks = (f + FF_BK(S) - 1) / FF_BK(S); g.segments = 2; g.a_parts = g.b_parts = 2; g.b_mn = 1;
+    g.M = m; g.N = d; g.k_blocks = ffn_k_blocks(S, f); g.segments = 2; g.a_parts = g.b_parts = 2; g.b_mn = 1;
     if ((rc = ffn_plain(S, g, oz, oi, dx, dt, partial, st))) return rc;
   }
   if (dw_in != nullptr) {
     g = base;
-    g.M = f; g.N = d; g.k_blocks = (m + FF_BK(S) - 1) / FF_BK(S); g.m_parts = g.a_parts = 2; g.a_mn = g.b_mn = 1;
+    g.M = f; g.N = d; g.k_blocks = ffn_k_blocks(S, m); g.m_parts = g.a_parts = 2; g.a_mn = g.b_mn = 1;
     if ((rc = ffn_plain(S, g, oz, ox, dw_in, dt, partial, st))) return rc;
   }
   if (dw_out != nullptr) {
     g = base;
-    g.M = n; g.N = f; g.k_blocks = (m + FF_BK(S) - 1) / FF_BK(S); g.a_mn = g.b_mn = 1;
+    g.M = n; g.N = f; g.k_blocks = ffn_k_blocks(S, m); g.a_mn = g.b_mn = 1;
     if ((rc = ffn_plain(S, g, oy, oh, dw_out, dt, partial, st))) return rc;
   }
   return 0;
