@@ -11,8 +11,8 @@
 //   plain   the four others
 // No operand is ever transposed in memory: a tile is fetched K-major or MN-major, whichever way the tensor lies.
 //
-// Pipeline: one TMA thread, one thread that issues tcgen05.mma (kind::f16, fp32 accumulators in TMEM), eight epilogue
-// warps; operands in a ring of 128-byte-swizzled stages of 64 k, accumulators double-buffered so that the epilogue of a tile
+// Pipeline: one TMA thread, one thread that issues tcgen05.mma (kind::f16, fp32 accumulators in TMEM), eight or
+// sixteen epilogue warps; operands in a ring of 128-byte-swizzled stages of 64 k, accumulators double-buffered so that the epilogue of a tile
 // runs under the multiplications of the next (persistent CTAs).  Large products run as pairs of CTAs (cta_group::2, 256-row
 // tiles): each CTA fetches half of the B tile, which halves its share of the operand traffic.
 //
@@ -31,8 +31,8 @@
 
 #define FF_BM 128            // accumulator rows of one CTA
 #define FF_BK(S) ((S) == 3 ? 32 : 64)    // k per stage: K-major rows of 64 (three planes) or 128 bytes = one swizzle row
-#define FF_EPI 8             // epilogue warps 0-7 (warp 0 owns TMEM), warp 8 TMA, warp 9 MMA
-#define FF_THREADS (32 * (FF_EPI + 2))
+// epilogue warps 0 .. EPI - 1 (warp 0 owns TMEM), then the TMA warp and the MMA warp
+#define FF_THREADS(EPI) (32 * ((EPI) + 2))
 
 #define FF_GATE 0
 #define FF_DGATE 1
@@ -168,6 +168,7 @@ __device__ __forceinline__ void tmem_wait16(float* v) {
                : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
                  "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
+template <int EPI>
 __device__ __forceinline__ bool ff_epi_bar_or(bool flag) {
   uint32_t r;
   asm volatile(
@@ -175,7 +176,7 @@ __device__ __forceinline__ bool ff_epi_bar_or(bool flag) {
       "setp.ne.u32 q, %1, 0;\n\t"
       "bar.red.or.pred p, 1, %2, q;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r) : "r"((uint32_t)flag), "n"(FF_EPI * 32) : "memory");
+      : "=r"(r) : "r"((uint32_t)flag), "n"(EPI * 32) : "memory");
   return r != 0;
 }
 
@@ -391,13 +392,17 @@ __device__ __forceinline__ void ff_load_z(const float* z, long long z_plane, boo
 
 // BN accumulator columns, S operand planes, CG CTAs per tile: a pair (CG = 2) shares one 256-row tile, each CTA fetches its
 // 128 rows of A and half of the B tile, so a byte of B serves 256 rows
-template <int BN, int S, int CG> struct FfnSmem {
+template <int BN, int S, int KIND, int CG> struct FfnSmem {
+  // Epilogue warps.  Three planes: the sums of a tile end in the epilogue's registers, so it does not run under the next tile;
+  // with sixteen warps its activation and splitting take less (1120 x 650 x 2600, gate 51.8 -> 47.8 us, dgate 52.4 -> 44.8).
+  // 16-bit operands: eight (dgate at 8192 x 2048 x 8192: 259 us, with sixteen and no room to fetch ahead 273).
+  static constexpr int EPI = S == 3 && (KIND == FF_DGATE || (KIND == FF_GATE && BN >= 128)) ? 16 : 8;
   static constexpr int A_TILE = FF_BM * FF_BK(S) * 2, B_TILE = BN / CG * FF_BK(S) * 2;
   static constexpr int STAGE = S * (A_TILE + B_TILE);
-  static constexpr int EPI = FF_EPI * 4096;               // 4 KB for each epilogue warp
-  static constexpr int ROOM = 227 * 1024 - 256 - 1024 - EPI;
+  static constexpr int EPI_BYTES = EPI * 4096;            // 4 KB for each epilogue warp
+  static constexpr int ROOM = 227 * 1024 - 256 - 1024 - EPI_BYTES;
   static constexpr int STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
-  static constexpr int BYTES = STAGES * STAGE + EPI + 256 + 1024;
+  static constexpr int BYTES = STAGES * STAGE + EPI_BYTES + 256 + 1024;
 };
 
 // Tile order: groups of FF_GROUP row tiles, rows fastest within a group, so that the tiles worked on at one time form a
@@ -434,14 +439,14 @@ __device__ __forceinline__ void ff_slice(const FfnGemm& g, int tile, int out_til
 }
 
 template <int BN, int S, int KIND, int CG>
-__global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_constant__ FfnGemm g) {
-  typedef FfnSmem<BN, S, CG> L;
+__global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1) ffn_gemm_kernel(const __grid_constant__ FfnGemm g) {
+  typedef FfnSmem<BN, S, KIND, CG> L;
   extern __shared__ uint8_t smem_raw[];
   // 1024-byte alignment: the swizzle pattern is a function of the shared-memory address bits
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int BK = FF_BK(S), CHUNK = 64 / BK;     // S = 3: an accumulator holds 64 k
   uint8_t* epi_smem = smem + L::STAGES * L::STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(epi_smem + L::EPI);   // CG = 2: the leader's count both CTAs' bytes
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi_smem + L::EPI_BYTES);   // CG = 2: the leader's count both CTAs' bytes
   uint64_t* empty = full + L::STAGES;
   uint64_t* acc_full = empty + L::STAGES;    // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2], the leader's
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full + b, 1);
-      mbar_init(acc_empty + b, FF_EPI * CG);   // one arrival per epilogue warp
+      mbar_init(acc_empty + b, L::EPI * CG);   // one arrival per epilogue warp
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
 
   // The TMA and the MMA warp run their loops as whole warps and elect a lane for the instructions alone: addresses and
   // descriptors then stay in uniform registers.
-  if (warp == FF_EPI) {
+  if (warp == L::EPI) {
     // ---------------- TMA producer ----------------
     uint32_t it = 0, s = 0, phase = 1;      // stage and the parity of its `empty` barrier (the first round passes at once)
     bool ok = true;
@@ -543,7 +548,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
       if (rank == 0)
         for (uint32_t j = it > L::STAGES ? it - L::STAGES : 0; j < it; ++j) mbar_wait(full + j % L::STAGES, (j / L::STAGES) & 1);
     }
-  } else if (warp == FF_EPI + 1 && rank == 0) {
+  } else if (warp == L::EPI + 1 && rank == 0) {
     // ---------------- MMA issuer (of a pair: the leader's) ----------------
     // instruction descriptor: fp32 accumulate, operand type, majorness bits, N >> 3, M >> 4
     const uint32_t type = g.fp16 ? 0u : 1u;
@@ -595,9 +600,9 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
       }
     }
     if (!ok) *abort_flag = 1;
-  } else if (warp < FF_EPI) {
-    // ---------------- epilogue: warp w reads lanes 32 (w % 4) ... of half of the tile's output columns ----------------
-    constexpr int HC = BN_OUT / 2;         // output columns per warp
+  } else if (warp < L::EPI) {
+    // ---------------- epilogue: warp w reads lanes 32 (w % 4) ... of its share of the tile's output columns ----------------
+    constexpr int HC = BN_OUT / (L::EPI / 4);         // output columns per warp
     const int half = warp >> 2;
     uint32_t chunk = 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -622,7 +627,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
         for (int i = 0; i < n_chunks; ++i, ++chunk) {
           const uint32_t buf = chunk & 1;
           const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
-          if (ff_epi_bar_or(bad)) { stop = true; break; }
+          if (ff_epi_bar_or<L::EPI>(bad)) { stop = true; break; }
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < NA; c += 32) {
@@ -662,7 +667,7 @@ __global__ void __launch_bounds__(FF_THREADS, 1) ffn_gemm_kernel(const __grid_co
         float zg[16], zu[16], yg[16], yu[16];
         if (KIND == FF_DGATE) ff_load_z(z, g.z_plane, 0 < z_cols, zg, zu);
         const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
-        if (ff_epi_bar_or(bad)) stop = true;
+        if (ff_epi_bar_or<L::EPI>(bad)) stop = true;
         else {
           tc_fence_after();
           ff_for_act<KIND>(g.act, [&](auto act) {
@@ -835,7 +840,8 @@ static int ffn_map(CUtensorMap* map, const FfnOperand& o, int fp16, int mn_major
 template <int BN, int S, int KIND, int CG>
 static int ffn_launch_t(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
   void (*kernel)(FfnGemm) = ffn_gemm_kernel<BN, S, KIND, CG>;
-  constexpr int smem = FfnSmem<BN, S, CG>::BYTES;
+  typedef FfnSmem<BN, S, KIND, CG> L;
+  constexpr int smem = L::BYTES;
   // before the tensor maps: a runtime call makes the device's context current in a thread that has not used it yet
   // (autograd's), without which the driver refuses to encode a map
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -851,7 +857,7 @@ static int ffn_launch_t(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cu
   const int most = sm_count() / CG, grid = CG * (tiles < most ? (int)tiles : most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(FF_THREADS);
+  cfg.blockDim = dim3(FF_THREADS(L::EPI));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -888,7 +894,7 @@ static double ffn_cost(const FfnTile& t, int S, int kind, int M, int m_parts, in
   const double rounds = (double)(long long)((tiles + sms - 1) / sms);
   const double mul = 2.0 * t.bn * (S == 3 ? 6 : 1), fetch = S * (FF_BM + t.bn / t.cg) * 128.0 / 58.0;
   const double step = mul > fetch ? mul : fetch, main = (double)((k64 + t.splits - 1) / t.splits) * step;
-  const double epi = t.bn * (kind == FF_DGATE ? 70.0 : 45.0);
+  const double epi = t.bn * (kind == FF_DGATE ? (S == 3 ? 180.0 : 70.0) : 45.0);
   double c = S == 3 ? rounds * (main + epi) : rounds * (main > epi ? main : epi) + epi;
   c += 3000.0;                                               // launch, first loads
   if (t.splits > 1) c += 5000.0 + 8.0 * t.splits * m_parts * M * cols / (30.0 * sm_count());
