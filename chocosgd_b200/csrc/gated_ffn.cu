@@ -27,7 +27,7 @@
 // Every mbarrier wait is bounded; a wait that runs out sets the error word, the CTA drains and frees its TMEM.
 #include "launch.cuh"
 #include "tc_common.cuh"
-#include "vec.cuh"
+#include "ffn.cuh"
 
 #define FF_BM 128            // accumulator rows of one CTA
 #define FF_BK(S) ((S) == 3 ? 32 : 64)    // k per stage: K-major rows of 64 (three planes) or 128 bytes = one swizzle row
@@ -38,11 +38,6 @@
 #define FF_DGATE 1
 #define FF_PLAIN 2
 #define FF_PARTIAL 3         // plain, over a part of k, into fp32 slices that ffn_join_kernel adds up
-
-#define ACT_SILU 0
-#define ACT_GELU 1
-#define ACT_RELU 2
-#define ACT_SIGMOID 3
 
 __device__ int g_ffn_error;
 
@@ -208,33 +203,6 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t (&q)[3]) {
     x -= __uint_as_float(q[s] << 16);
     y -= __uint_as_float(q[s] & 0xFFFF0000u);
   }
-}
-
-// activation and (wanted) its derivative.  The reciprocal is the approximate one (1 unit of the last place); FAST: so is the
-// exponential (relative error |z| 2^-23), which suits 16-bit results.
-template <int ACT, bool GRAD, bool FAST>
-__device__ __forceinline__ float ff_act(float z, float& slope) {
-  if (ACT == ACT_GELU) {
-    const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    if (GRAD) {
-      const float e = -0.5f * z * z;
-      slope = fmaf(z * 0.39894228040143268f, FAST ? __expf(e) : expf(e), cdf);
-    }
-    return z * cdf;
-  }
-  if (ACT == ACT_RELU) {
-    if (GRAD) slope = z > 0.f ? 1.f : 0.f;
-    return z < 0.f ? 0.f : z;
-  }
-  float sg;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(sg) : "f"(1.f + (FAST ? __expf(-z) : expf(-z))));
-  if (ACT == ACT_SILU) {
-    const float a = z * sg;
-    if (GRAD) slope = fmaf(a, 1.f - sg, sg);
-    return a;
-  }
-  if (GRAD) slope = fmaf(-sg, sg, sg);
-  return sg;
 }
 
 // ---- a warp's 32 rows x up to 128 bytes through shared memory, so that rows are written as whole lines -----------------
@@ -1014,14 +982,19 @@ extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt
   return a > c ? a : c;
 }
 
+// most tokens of an evaluation pass that the form for few tokens takes (`few` of gated_ffn_forward)
+extern "C" int gated_ffn_few_tokens(int dt) { return ffn_few_tokens(dt); }
+
+// few: no operand images, no partial sums and no z; h: m x pad16(f) fp32.  Else:
 // Every operand comes with an optional image: [S][rows][pad16(cols)] 16-bit elements, S = 3 for fp32, needed for fp32 and
 // for rows that do not start on 16-byte boundaries.  h: [S][m][pad16(f)] 16-bit; z: 2 x (m rounded up to 32) x pad16(f) fp32 or null;
 // partial: gated_ffn_partial_floats.
 extern "C" int gated_ffn_forward(const void* x, long long ldx, void* x_img, const void* w_in, long long ld_in, void* in_img,
                                  const void* w_out, long long ld_out, void* out_img, void* h, float* z, float* partial, void* y,
-                                 int m, int d, int f, int n, int act, int dt, cudaStream_t st) {
+                                 int m, int d, int f, int n, int act, int dt, int few, cudaStream_t st) {
   const FfnShape s = {m, d, f, n, act, dt};
   if (!ffn_shape_ok(s)) return -1;
+  if (few) return ffn_few_forward(x, ldx, w_in, ld_in, w_out, ld_out, reinterpret_cast<float*>(h), y, m, d, f, n, act, dt, st);
   FfnOperand ox, oi, oo;
   FfnImages images = {};
   ffn_prepare(&ox, x, m, d, ldx, 1, dt, x_img, &images);

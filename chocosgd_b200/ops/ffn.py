@@ -21,9 +21,11 @@ def _declare():
     lib = _lib.load()
     if not getattr(lib, "_ffn_declared", False):
         vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        lib.gated_ffn_forward.argtypes = [vp, ll, vp] * 3 + [vp] * 4 + [i] * 6 + [vp]
+        lib.gated_ffn_forward.argtypes = [vp, ll, vp] * 3 + [vp] * 4 + [i] * 7 + [vp]
         lib.gated_ffn_backward.argtypes = [vp, ll, vp] * 4 + [vp] * 7 + [i] * 6 + [vp]
         lib.gated_ffn_forward.restype = lib.gated_ffn_backward.restype = lib.gated_ffn_last_error.restype = i
+        lib.gated_ffn_few_tokens.argtypes = [i]
+        lib.gated_ffn_few_tokens.restype = i
         lib.gated_ffn_partial_floats.argtypes = [i] * 6
         lib.gated_ffn_partial_floats.restype = ll
         lib._ffn_declared = True
@@ -80,21 +82,25 @@ class _GatedFfnFn(torch.autograd.Function):
         (m, d), f, n = x2.shape, w_in.shape[0] // 2, w_out.shape[0]
         train = any(ctx.needs_input_grad)
         y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+        dt = DT[x.dtype]
+        few = not train and m <= lib.gated_ffn_few_tokens(dt)
         lay = _Layout()
-        img = [lay.image(t) for t in (x2, wi, wo)]
-        planes = 3 if x.dtype == torch.float32 else 1
-        h = lay.add(planes * m * _pad16(f) * 2)
-        z = lay.add(2 * _pad32(m) * _pad16(f) * 4) if train else None
-        partial = lay.scratch(lib.gated_ffn_partial_floats(m, d, f, n, DT[x.dtype], 0))
+        if few:
+            img, z, partial, h = (None, None, None), None, None, lay.add(4 * m * _pad16(f))
+        else:
+            img = [lay.image(t) for t in (x2, wi, wo)]
+            h = lay.add((3 if x.dtype == torch.float32 else 1) * m * _pad16(f) * 2)
+            z = lay.add(2 * _pad32(m) * _pad16(f) * 4) if train else None
+            partial = lay.scratch(lib.gated_ffn_partial_floats(m, d, f, n, dt, 0))
         buf = torch.empty(lay.size, dtype=torch.uint8, device=x.device)
         if m:
             b = buf.data_ptr()
             rc = lib.gated_ffn_forward(x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
-                                       wo.data_ptr(), wo.stride(0), _at(b, img[2]), b + h, _at(b, z), _at(b, partial), y.data_ptr(), m, d, f,
-                                       n, act, DT[x.dtype], _lib.stream_ptr())
+                                       wo.data_ptr(), wo.stride(0), _at(b, img[2]), b + h, _at(b, z), _at(b, partial),
+                                       y.data_ptr(), m, d, f, n, act, dt, int(few), _lib.stream_ptr())
             if rc:
                 raise RuntimeError(f"gated_ffn_forward failed with code {rc}")
-            _lib.count(2 + sum(i is not None for i in img))
+            _lib.count(2 + int(any(i is not None for i in img)) + int(partial is not None))
         if train:
             ctx.save_for_backward(x2, wi, wo, buf)
             ctx.layout, ctx.act, ctx.x_shape = (img, h, z), act, x.shape
