@@ -3,21 +3,27 @@
 //   mu = mean(x), var = mean((x - mu)^2), rs = 1 / sqrt(var + eps), z = (x - mu) rs, y = z w + b
 //   g = dy w;  dx = rs (g - mean(g) - z mean(g z));  dw = sum over rows of dy z;  db = sum over rows of dy
 //
-// Both directions are one pass over memory: a row is read once, held in registers (the variance is taken about the
-// mean, not from a sum of squares) and written once.  A row belongs to a group of T = 32 .. 1024 threads with E = 8
-// consecutive-vector elements each (16 for rows above 8192); a block holds several groups and walks over the rows, so
-// that weight and bias are fetched once per block.  All statistics and sums are fp32.
+// Both directions are one pass over memory: a row is read once, kept on the SM (the variance is taken about the mean, not from
+// a sum of squares) and written once.  All statistics and sums are fp32.
 //
-// The backward kernel keeps the running sums of dw and db of its columns in registers over all rows of its block,
-// adds the block's groups in shared memory and writes one partial row per block; a second kernel adds the partial
-// rows in block order.  No atomics: the same inputs give the same bits.
+// Forward: a row belongs to one warp (up to 64 bytes x 16 per lane as they lie in memory, no block barrier), to several for long
+// rows and where there are few rows; blocks walk over the rows with weight and bias in shared memory.
 //
-// Rows that do not start on 16-byte (8- / 4-byte) boundaries take narrower accesses (V elements at a time); rows
-// too long for registers (above 16384 elements) take the *_long kernels, which read the row again from L2.
+// Backward: a row belongs to a group of 32 .. 1024 threads, so that a thread's share of the columns is small enough to keep
+// the running sums of dw and db of all its rows in registers.  Rows that start on 16-byte boundaries come through a ring of
+// bulk copies in shared memory (three rows of x and dy per group under way); others are read into registers.  A block adds its
+// groups in shared memory and writes one partial row; a second kernel adds the partial rows in block order.  No atomics: the same
+// inputs give the same bits.
+//
+// Rows that do not start on 16-byte boundaries take narrower accesses (V elements at a time); rows too long for registers
+// (above 16384 elements) take the *_long kernels, which read the row again from L2.
 #include "launch.cuh"
+#include "tc_common.cuh"
 #include "vec.cuh"
 
 #define LN_MAX_ROW 16384
+
+__device__ int g_ln_error;      // a bounded wait ran out
 
 struct LnArgs {
   const void* x;        // [N, D], ldx elements per row
@@ -77,51 +83,222 @@ __device__ __forceinline__ void ln_load(const T* row, int d, int t, int threads,
   }
 }
 
-template <typename T, int V, int E>
-__global__ void __launch_bounds__(1024) ln_fwd_kernel(LnArgs a, int threads, int groups) {
-  __shared__ float red[32][2][32];   // [group][buffer][warp]
-  const int group = threadIdx.x / threads, t = threadIdx.x % threads;
+// value `c` of a parameter (`none` without it)
+__device__ __forceinline__ float ln_param(const void* p, int dt, int c, float none) {
+  return p != nullptr ? load_any(p, dt, c) : none;
+}
+// parameters wait in shared memory as fp32 in four-element pieces: piece h of vector v at (h vectors + v), so that consecutive
+// lanes read consecutive 16-byte units
+template <int V>
+__device__ __forceinline__ void ln_get(const float* s, int vectors, int v, float (&out)[V]) {
+  if (V >= 4) {
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+      const float4 q = reinterpret_cast<const float4*>(s)[h * vectors + v];
+      out[(4 * h) % V] = q.x; out[(4 * h + 1) % V] = q.y; out[(4 * h + 2) % V] = q.z; out[(4 * h + 3) % V] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = s[v * V + k];
+  }
+}
+template <int V>
+__device__ __forceinline__ int ln_slot(int vectors, int c) {      // where element c is kept
+  return V >= 4 ? ((c % V / 4) * vectors + c / V) * 4 + c % 4 : c;
+}
+
+// Rows of up to 32 V NV elements per warp.  16384 x 4096 bf16: see the kernel's figures in the launch code.
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(256, NV >= 16 ? 2 : 4) ln_fwd_kernel(LnArgs a, int threads, int groups) {
+  extern __shared__ float4 ln_smem4[];
+  float *w_s = reinterpret_cast<float*>(ln_smem4), *b_s = w_s + (a.d + V - 1) / V * V;
+  __shared__ float red[8][2][32];   // [group][buffer][warp]
+  const int group = threadIdx.x / threads, t = threadIdx.x % threads, vectors = (a.d + V - 1) / V;
   pdl_wait();
   pdl_trigger();
-  float w[E], b[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = ln_col<V>(t, threads, e);
-    w[e] = c < a.d && a.w != nullptr ? load_any(a.w, a.w_dt, c) : 1.f;
-    b[e] = c < a.d && a.b != nullptr ? load_any(a.b, a.w_dt, c) : 0.f;
-  }
+  const T* x = reinterpret_cast<const T*>(a.x);
   const float inv_d = 1.f / (float)a.d;
-  for (long long row = (long long)blockIdx.x * groups + group; row < a.n; row += (long long)gridDim.x * groups) {
-    float x[E];
-    ln_load<T, V, E>(reinterpret_cast<const T*>(a.x) + row * a.ldx, a.d, t, threads, x);
+  const long long first = (long long)blockIdx.x * groups + group, stride = (long long)gridDim.x * groups;
+  Vec<T, V> r[NV];
+  const auto load = [&](long long row) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      r[j].clear();
+      if (j * threads + t < vectors) r[j].load(x + row * a.ldx + (j * threads + t) * V);
+    }
+  };
+  if (first < a.n) load(first);
+  for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+    w_s[ln_slot<V>(vectors, c)] = ln_param(a.w, a.w_dt, c, 1.f);
+    b_s[ln_slot<V>(vectors, c)] = ln_param(a.b, a.w_dt, c, 0.f);
+  }
+  __syncthreads();
+  for (long long row = first; row < a.n; row += stride) {
+    if (row != first) load(row);
     float s[1] = {0.f};
 #pragma unroll
-    for (int e = 0; e < E; ++e) s[0] += x[e];
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) s[0] += to_f(r[j].e[k]);
     ln_group_sum<1>(s, red[group][0], group, t, threads);
     const float mu = s[0] * inv_d;
     s[0] = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] -= mu;
-      if (ln_col<V>(t, threads, e) < a.d) s[0] = fmaf(x[e], x[e], s[0]);
-    }
+    for (int j = 0; j < NV; ++j) opaque(r[j].raw);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (j * threads + t < vectors) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float v = to_f(r[j].e[k]) - mu;
+          s[0] = fmaf(v, v, s[0]);
+        }
+      }
     ln_group_sum<1>(s, red[group][1], group, t, threads);
     const float rs = 1.f / sqrtf(fmaf(s[0], inv_d, a.eps));
     T* y = reinterpret_cast<T*>(a.y) + row * a.d;
 #pragma unroll
-    for (int j = 0; j < E / V; ++j) {
-      const int c = (j * threads + t) * V;
-      if (c >= a.d) continue;
-      Vec<T, V> v;
+    for (int j = 0; j < NV; ++j) opaque(r[j].raw);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v.e[k] = from_f<T>(fmaf(x[j * V + k] * rs, w[j * V + k], b[j * V + k]));
-      v.store(y + c);
-    }
+    for (int j = 0; j < NV; ++j)
+      if (j * threads + t < vectors) {
+        float w[V], b[V];
+        ln_get<V>(w_s, vectors, j * threads + t, w);
+        ln_get<V>(b_s, vectors, j * threads + t, b);
+        Vec<T, V> o;
+#pragma unroll
+        for (int k = 0; k < V; ++k) o.e[k] = from_f<T>(fmaf((to_f(r[j].e[k]) - mu) * rs, w[k], b[k]));
+        o.store(y + (j * threads + t) * V);
+      }
     if (t == 0 && a.mean != nullptr) {
       a.mean[row] = mu;
       a.rstd[row] = rs;
     }
   }
+}
+
+#define LN_RING 3        // rows of a group under way
+
+__device__ __forceinline__ void ln_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// Rows on 16-byte boundaries.  x and dy of a row lie in a stage of the group's ring and are read there twice, before and after
+// the row's two sums are known; registers hold only the sums of dw and db (32 at 16 elements per thread, 1024 threads).  The stage
+// of the row before is filled again behind the barrier of the row's sums: by then every thread is done with it.
+template <typename T, int E>
+__global__ void __launch_bounds__(1024, 1) ln_bwd_ring_kernel(LnArgs a, int threads, int groups) {
+  constexpr int V = 16 / sizeof(T), NV = E / V;
+  extern __shared__ float4 ln_smem4[];
+  __shared__ float red[16][2][64];
+  __shared__ uint64_t full[16][LN_RING];
+  const int vectors = a.d / V, row_bytes = vectors * 16;
+  float* w_s = reinterpret_cast<float*>(ln_smem4);                       // [D], later [2][D] sums of the block's groups
+  uint8_t* ring = reinterpret_cast<uint8_t*>(ln_smem4) + (a.d * 8 + 15) / 16 * 16;
+  const int group = threadIdx.x / threads, t = threadIdx.x % threads;
+  uint8_t* mine = ring + (long long)group * LN_RING * 2 * row_bytes;
+  if (t == 0) {
+    for (int k = 0; k < LN_RING; ++k) mbar_init(&full[group][k], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+  const T *x = reinterpret_cast<const T*>(a.x), *dy = reinterpret_cast<const T*>(a.dy);
+  for (int c = threadIdx.x; c < a.d; c += blockDim.x) w_s[ln_slot<V>(vectors, c)] = ln_param(a.w, a.w_dt, c, 1.f);
+  __syncthreads();
+  const long long first = (long long)blockIdx.x * groups + group, stride = (long long)gridDim.x * groups;
+  const auto fill = [&](long long row, int k) {
+    mbar_expect_tx(&full[group][k], 2 * row_bytes);
+    ln_bulk(mine + k * 2 * row_bytes, x + row * a.ldx, row_bytes, &full[group][k]);
+    ln_bulk(mine + k * 2 * row_bytes + row_bytes, dy + row * a.lddy, row_bytes, &full[group][k]);
+  };
+  if (t == 0)
+    for (int k = 0; k < LN_RING - 1; ++k)
+      if (first + k * stride < a.n) fill(first + k * stride, k);
+  float dw[E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
+  const float inv_d = 1.f / (float)a.d;
+  int turn = 0, k = 0;
+  uint32_t phase = 0;
+  float next_mu = first < a.n ? a.mean[first] : 0.f, next_rs = first < a.n ? a.rstd[first] : 0.f;
+  for (long long row = first; row < a.n; row += stride, turn ^= 1) {
+    const float mu = next_mu, rs = next_rs;
+    if (row + stride < a.n) {
+      next_mu = a.mean[row + stride];
+      next_rs = a.rstd[row + stride];
+    }
+    if (!mbar_wait(&full[group][k], phase)) atomicExch(&g_ln_error, 1);
+    const uint4 *xs = reinterpret_cast<const uint4*>(mine + k * 2 * row_bytes), *gs = xs + vectors;
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int v = j * threads + t;
+      if (v < vectors) {
+        Vec<T, V> px, pg;
+        px.load(reinterpret_cast<const T*>(xs + v));
+        pg.load(reinterpret_cast<const T*>(gs + v));
+        float w[V];
+        ln_get<V>(w_s, vectors, v, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float z = (to_f(px.e[e]) - mu) * rs, g = to_f(pg.e[e]), gw = g * w[e];
+          dw[j * V + e] = fmaf(g, z, dw[j * V + e]);
+          db[j * V + e] += g;
+          s[0] += gw;
+          s[1] = fmaf(gw, z, s[1]);
+        }
+      }
+    }
+    ln_group_sum<2>(s, red[group][turn], group, t, threads);
+    if (threads == 32) __syncwarp();
+    if (t == 0 && row + (LN_RING - 1) * stride < a.n) fill(row + (LN_RING - 1) * stride, (k + LN_RING - 1) % LN_RING);
+    if (a.dx != nullptr) {
+      const float mg = s[0] * inv_d, mgz = s[1] * inv_d;
+      T* dx = reinterpret_cast<T*>(a.dx) + row * a.d;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int v = j * threads + t;
+        if (v < vectors) {
+          Vec<T, V> px, pg, o;
+          px.load(reinterpret_cast<const T*>(xs + v));
+          pg.load(reinterpret_cast<const T*>(gs + v));
+          float w[V];
+          ln_get<V>(w_s, vectors, v, w);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float z = (to_f(px.e[e]) - mu) * rs;
+            o.e[e] = from_f<T>(rs * (fmaf(to_f(pg.e[e]), w[e], -mg) - z * mgz));
+          }
+          o.store(dx + v * V);
+        }
+      }
+    }
+    if (++k == LN_RING) { k = 0; phase ^= 1; }
+  }
+  if (a.partial == nullptr) return;
+  float* acc_s = w_s;
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * a.d; c += blockDim.x) acc_s[c] = 0.f;
+  for (int q = 0; q < groups; ++q) {
+    __syncthreads();
+    if (q != group) continue;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int v = j * threads + t;
+      if (v < vectors) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          acc_s[v * V + e] += dw[j * V + e];
+          acc_s[a.d + v * V + e] += db[j * V + e];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  float* out = a.partial + (long long)blockIdx.x * 2 * a.d;
+  for (int c = threadIdx.x; c < 2 * a.d; c += blockDim.x) out[c] = acc_s[c];
 }
 
 template <typename T, int V, int E>
@@ -135,7 +312,7 @@ __global__ void __launch_bounds__(1024, 1) ln_bwd_kernel(LnArgs a, int threads, 
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = ln_col<V>(t, threads, e);
-    w[e] = c < a.d && a.w != nullptr ? load_any(a.w, a.w_dt, c) : 1.f;
+    w[e] = c < a.d ? ln_param(a.w, a.w_dt, c, 1.f) : 1.f;
     dw[e] = db[e] = 0.f;
   }
   const float inv_d = 1.f / (float)a.d;
@@ -187,28 +364,30 @@ __global__ void __launch_bounds__(1024, 1) ln_bwd_kernel(LnArgs a, int threads, 
   for (int c = threadIdx.x; c < 2 * a.d; c += blockDim.x) out[c] = acc_s[c];
 }
 
-// dw | db: column sums of the partial rows in block order; eight slices of rows per column, then the slices in order
-__global__ void __launch_bounds__(256) ln_reduce_kernel(const float* partial, int blocks, int d, void* dw, void* db, int w_dt) {
-  __shared__ float s[8][33];
+// dw | db: column sums of the partial rows: 32 slices of rows per column (one warp each, all loads under way at once), then the
+// slices by a fixed tree
+__global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* partial, int blocks, int d, void* dw, void* db, int w_dt) {
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const long long c = (long long)blockIdx.x * 32 + lane;
   pdl_wait();
   pdl_trigger();
   float v = 0.f;
-  if (c < 2 * d) {
-    const int per = (blocks + 7) / 8, end = min(blocks, (slice + 1) * per);
+  if (c < 2LL * d) {
+    const int per = (blocks + 31) / 32, end = min(blocks, (slice + 1) * per);
+#pragma unroll 8
     for (int r = slice * per; r < end; ++r) v += partial[(long long)r * 2 * d + c];
   }
   s[slice][lane] = v;
   __syncthreads();
-  if (slice != 0 || c >= 2 * d) return;
-  v = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v += s[k][lane];
-  if (c < d) {
-    if (dw != nullptr) store_any(dw, w_dt, c, v);
+  // warp w sums column w over the slices
+  const long long mine = (long long)blockIdx.x * 32 + slice;
+  v = ln_warp_sum(s[lane][slice]);
+  if (lane != 0 || mine >= 2LL * d) return;
+  if (mine < d) {
+    if (dw != nullptr) store_any(dw, w_dt, mine, v);
   } else if (db != nullptr) {
-    store_any(db, w_dt, c - d, v);
+    store_any(db, w_dt, mine - d, v);
   }
 }
 
@@ -304,34 +483,64 @@ static int ln_threads(int d, int e) { return ((d + e - 1) / e + 31) / 32 * 32; }
 // blocks of the backward kernel = partial rows; one block per SM (its 1024 threads fill the register file)
 extern "C" long long layer_norm_partial_floats(int d) { return (long long)sm_count() * 2 * d; }
 
-template <typename T, int V, int E>
-static int ln_launch(const LnArgs& a, bool bwd, int* blocks, cudaStream_t st) {
-  const int threads = ln_threads(a.d, E);
+template <typename T, int V, int NV>
+static int ln_launch_fwd(const LnArgs& a, cudaStream_t st) {
+  const int threads = 32 * ((a.d + 32 * V * NV - 1) / (32 * V * NV));
+  int groups = 256 / threads;
+  if (threads > 256) return -1;
   const long long per_sm = (a.n + sm_count() - 1) / sm_count();
-  if (!bwd) {
-    // groups per block: about 256 threads, fewer when there are too few rows to give every SM a block
-    long long groups = threads >= 256 ? 1 : 256 / threads;
-    if (groups > per_sm) groups = per_sm;
-    long long blocks_f = (a.n + groups - 1) / groups;
-    const long long most = (long long)sm_count() * (2048 / (threads * groups < 32 ? 32 : threads * groups));
-    if (blocks_f > most) blocks_f = most;
-    return (int)launch_k(ln_fwd_kernel<T, V, E>, dim3((unsigned)blocks_f), dim3((unsigned)(threads * groups)), 0, st, a,
-                         threads, (int)groups);
+  if (groups > per_sm) groups = (int)per_sm;
+  long long blocks = (a.n + groups - 1) / groups;
+  // as many blocks as the registers of NV vectors leave room for, about
+  const long long most = (long long)sm_count() * (NV >= 16 ? 2 : 4) * (256 / (threads * groups));
+  if (blocks > most) blocks = most;
+  const int smem = 2 * (a.d + V - 1) / V * V * (int)sizeof(float) + 16;
+  void (*kernel)(LnArgs, int, int) = ln_fwd_kernel<T, V, NV>;
+  if (smem > 40 * 1024) {      // set for every launch: the attribute belongs to the current device
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
   }
+  return (int)launch_k(kernel, dim3((unsigned)blocks), dim3((unsigned)(threads * groups)), (size_t)smem, st, a, threads, groups);
+}
+// Vectors per lane: 16 when there are rows for eight warps on every SM (a row per warp needs no block barrier), and where the
+// row would not fit otherwise; else 4 or 2, so that more warps share a row's latency.
+template <typename T, int V>
+static int ln_fwd(const LnArgs& a, cudaStream_t st) {
+  if (a.d > 256 * V * 4 || (a.n >= 8LL * sm_count() && a.d > 32 * V * 4)) {
+    if (a.d > 256 * V * 16) return ln_launch_fwd<T, V, 64 / V>(a, st);      // element-wise rows: up to 64 per lane
+    return ln_launch_fwd<T, V, 16>(a, st);
+  }
+  if (a.d > 256 * V * 2) return ln_launch_fwd<T, V, 4>(a, st);
+  return ln_launch_fwd<T, V, 2>(a, st);
+}
+
+template <typename T, int V, int E, bool RING>
+static int ln_launch_bwd(const LnArgs& a, int* blocks, cudaStream_t st) {
+  const int threads = ln_threads(a.d, E);
+  if (threads > 1024) return -1;
+  const long long per_sm = (a.n + sm_count() - 1) / sm_count();
   long long groups = 1024 / threads;
   if (groups > 15 && threads > 32) groups = 15;     // named barriers 1 .. 15
+  if (RING && groups > 16) groups = 16;
   if (groups > per_sm) groups = per_sm;
+  long long smem = (a.partial != nullptr ? 2 : 0) * a.d * (long long)sizeof(float);
+  if (RING) {
+    const long long stage = 2LL * a.d * (long long)sizeof(T), fixed = (a.d * 8LL + 15) / 16 * 16;
+    while (groups > 1 && fixed + groups * LN_RING * stage > 200 * 1024) --groups;
+    smem = fixed + groups * LN_RING * stage;
+    if (smem > 200 * 1024) return -1;
+  }
   long long nb = (a.n + groups - 1) / groups;
   if (nb > sm_count()) nb = sm_count();
   *blocks = (int)nb;
-  const int smem = a.partial != nullptr ? 2 * a.d * (int)sizeof(float) : 0;
-  if (smem > 32 * 1024) {
-    // set for every launch: the attribute belongs to the current device
-    cudaError_t e = cudaFuncSetAttribute(ln_bwd_kernel<T, V, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  void (*kernel)(LnArgs, int, int) = nullptr;
+  if constexpr (RING) kernel = ln_bwd_ring_kernel<T, E>;
+  else kernel = ln_bwd_kernel<T, V, E>;
+  if (smem > 16 * 1024) {      // set for every launch: the attribute belongs to the current device
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
   }
-  return (int)launch_k(ln_bwd_kernel<T, V, E>, dim3((unsigned)nb), dim3((unsigned)(threads * groups)), (size_t)smem, st,
-                       a, threads, (int)groups);
+  return (int)launch_k(kernel, dim3((unsigned)nb), dim3((unsigned)(threads * groups)), (size_t)smem, st, a, threads, (int)groups);
 }
 
 template <typename T>
@@ -350,14 +559,20 @@ static int ln_dispatch(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStrea
   }
   const int v = ln_vec(a, dt, bwd);
   constexpr int W = 16 / sizeof(T);
-  if (a.d <= 8192) {
-    if (v == W) return ln_launch<T, W, 8>(a, bwd, blocks, st);
-    if (v == 2) return ln_launch<T, 2, 8>(a, bwd, blocks, st);
-    return ln_launch<T, 1, 8>(a, bwd, blocks, st);
+  if (!bwd) {
+    if (v == W) return ln_fwd<T, W>(a, st);
+    if (v == 2) return ln_fwd<T, 2>(a, st);
+    return ln_fwd<T, 1>(a, st);
   }
-  if (v == W) return ln_launch<T, W, 16>(a, bwd, blocks, st);
-  if (v == 2) return ln_launch<T, 2, 16>(a, bwd, blocks, st);
-  return ln_launch<T, 1, 16>(a, bwd, blocks, st);
+  // 16 elements per thread for 16-bit rows (two vectors; the sums' shuffles weigh half), 8 for fp32; the ring where its three rows fit
+  if (v == W) {
+    constexpr int E = sizeof(T) == 2 ? 16 : 8;
+    if ((long long)a.d * (8 + LN_RING * 2 * (long long)sizeof(T)) <= 200 * 1024 && a.d <= 1024 * E)
+      return ln_launch_bwd<T, W, E, true>(a, blocks, st);
+    return a.d <= 8192 ? ln_launch_bwd<T, W, 8, false>(a, blocks, st) : ln_launch_bwd<T, W, 16, false>(a, blocks, st);
+  }
+  if (v == 2) return a.d <= 8192 ? ln_launch_bwd<T, 2, 8, false>(a, blocks, st) : ln_launch_bwd<T, 2, 16, false>(a, blocks, st);
+  return a.d <= 8192 ? ln_launch_bwd<T, 1, 8, false>(a, blocks, st) : ln_launch_bwd<T, 1, 16, false>(a, blocks, st);
 }
 
 static int ln_run(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStream_t st) {
@@ -388,6 +603,13 @@ extern "C" int layer_norm_backward(const void* x, long long ldx, const void* dy,
   int blocks = 0;
   int rc = ln_run(a, dt, true, &blocks, st);
   if (rc || partial == nullptr) return rc;
-  return (int)launch_k(ln_reduce_kernel, dim3((unsigned)((2LL * d + 31) / 32)), dim3(256), 0, st, (const float*)partial,
+  return (int)launch_k(ln_reduce_kernel, dim3((unsigned)((2LL * d + 31) / 32)), dim3(1024), 0, st, (const float*)partial,
                        blocks, d, dw, db, w_dt);
+}
+
+// 0, or 1 after a bounded wait of the backward kernel on the current device ran out (synchronises)
+extern "C" int layer_norm_last_error() {
+  int v = -1;
+  cudaMemcpyFromSymbol(&v, g_ln_error, sizeof(int));
+  return v;
 }

@@ -17,6 +17,12 @@ template <> struct RawVec<8> { typedef uint2 type; };
 template <> struct RawVec<4> { typedef uint32_t type; };
 template <> struct RawVec<2> { typedef uint16_t type; };
 
+// hides a value's origin from the compiler, which else keeps conversions of it alive instead of doing them again
+__device__ __forceinline__ void opaque(uint4& v) { asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)); }
+__device__ __forceinline__ void opaque(uint2& v) { asm volatile("" : "+r"(v.x), "+r"(v.y)); }
+__device__ __forceinline__ void opaque(uint32_t& v) { asm volatile("" : "+r"(v)); }
+__device__ __forceinline__ void opaque(uint16_t& v) { asm volatile("" : "+h"(v)); }
+
 // V elements of T as they lie in memory
 template <typename T, int V> struct Vec {
   typedef typename RawVec<sizeof(T) * V>::type Raw;
