@@ -123,13 +123,21 @@ static int dropout_launch(const void* x, const void* res, void* y, long long n, 
 }
 
 // y[i] = res[i] + keep(i) x[i] 65536 / (65536 - drop), i < n; res may be null; key: 8 bytes on the device;
-// drop = 0 .. 65535 (65536, everything dropped, is the caller's)
-extern "C" int dropout_apply(const void* x, const void* res, void* y, long long n, const void* key, unsigned site,
-                             unsigned drop, int dt, cudaStream_t st) {
-  if (n <= 0 || drop > 65535u || ((uintptr_t)key & 3) != 0) return -1;
-  const float scale = 65536.f / (65536.f - (float)drop);
-  if (dt == DT_F32) return dropout_launch<float>(x, res, y, n, key, site, drop, scale, st);
-  if (dt == DT_BF16) return dropout_launch<__nv_bfloat16>(x, res, y, n, key, site, drop, scale, st);
-  if (dt == DT_F16) return dropout_launch<__half>(x, res, y, n, key, site, drop, scale, st);
+// drop = 0 .. 65535 (65536, everything dropped, is the caller's).  The call takes one struct of 8-byte members.
+struct DropoutCall {
+  const void *x, *res;
+  void* y;
+  long long n;
+  const void* key;
+  long long site, drop, dt;
+  cudaStream_t stream;
+};
+extern "C" int dropout_apply(const DropoutCall* c) {
+  if (c->n <= 0 || c->drop < 0 || c->drop > 65535 || ((uintptr_t)c->key & 3) != 0) return -1;
+  const float scale = 65536.f / (65536.f - (float)c->drop);
+  const uint32_t site = (uint32_t)c->site, drop = (uint32_t)c->drop;
+  if (c->dt == DT_F32) return dropout_launch<float>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, c->stream);
+  if (c->dt == DT_BF16) return dropout_launch<__nv_bfloat16>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, c->stream);
+  if (c->dt == DT_F16) return dropout_launch<__half>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, c->stream);
   return -1;
 }

@@ -876,7 +876,8 @@ static FfnTile ffn_tile_for(int S, int kind, int M, int m_parts, int cols, long 
   double cost = 1e300;
   for (int i = 0; i < 4; ++i) {
     if (shapes[i].cg == 2 && M <= FF_BM) continue;
-    for (int q = 1; q <= (kind == FF_PLAIN && (i == 1 || i == 3) ? 16 : 1); ++q) {
+    // 1, 2, 3, 4, 6, 8, 12, 16 slices
+    for (int q = 1; q <= (kind == FF_PLAIN && (i == 1 || i == 3) ? 16 : 1); q += q < 4 ? 1 : (q < 8 ? 2 : 4)) {
       if (q > 1 && (k64 / q < 4 || (long long)m_parts * ((M + 31) / 32) > 65535)) break;    // 65535: grid of ffn_join_kernel
       FfnTile t = shapes[i];
       t.splits = q;
@@ -989,12 +990,31 @@ extern "C" int gated_ffn_few_tokens(int dt) { return ffn_few_tokens(dt); }
 // Every operand comes with an optional image: [S][rows][pad16(cols)] 16-bit elements, S = 3 for fp32, needed for fp32 and
 // for rows that do not start on 16-byte boundaries.  h: [S][m][pad16(f)] 16-bit; z: 2 x (m rounded up to 32) x pad16(f) fp32 or null;
 // partial: gated_ffn_partial_floats.
-extern "C" int gated_ffn_forward(const void* x, long long ldx, void* x_img, const void* w_in, long long ld_in, void* in_img,
-                                 const void* w_out, long long ld_out, void* out_img, void* h, float* z, float* partial, void* y,
-                                 int m, int d, int f, int n, int act, int dt, int few, cudaStream_t st) {
+struct FfnForwardCall {          // the calls take one struct of 8-byte members
+  const void* x;
+  long long ldx;
+  void* x_img;
+  const void* w_in;
+  long long ld_in;
+  void* in_img;
+  const void* w_out;
+  long long ld_out;
+  void *out_img, *h;
+  float *z, *partial;
+  void* y;
+  long long m, d, f, n, act, dt, few;
+  cudaStream_t st;
+};
+extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
+  const void *x = c->x, *w_in = c->w_in, *w_out = c->w_out;
+  void *x_img = c->x_img, *in_img = c->in_img, *out_img = c->out_img, *h = c->h, *y = c->y;
+  float *z = c->z, *partial = c->partial;
+  const long long ldx = c->ldx, ld_in = c->ld_in, ld_out = c->ld_out;
+  const int m = (int)c->m, d = (int)c->d, f = (int)c->f, n = (int)c->n, act = (int)c->act, dt = (int)c->dt;
+  const cudaStream_t st = c->st;
   const FfnShape s = {m, d, f, n, act, dt};
   if (!ffn_shape_ok(s)) return -1;
-  if (few) return ffn_few_forward(x, ldx, w_in, ld_in, w_out, ld_out, reinterpret_cast<float*>(h), y, m, d, f, n, act, dt, st);
+  if (c->few) return ffn_few_forward(x, ldx, w_in, ld_in, w_out, ld_out, reinterpret_cast<float*>(h), y, m, d, f, n, act, dt, st);
   FfnOperand ox, oi, oo;
   FfnImages images = {};
   ffn_prepare(&ox, x, m, d, ldx, 1, dt, x_img, &images);
@@ -1020,10 +1040,35 @@ extern "C" int gated_ffn_forward(const void* x, long long ldx, void* x_img, cons
 
 // x, w_in, w_out: as in the forward pass; where an image is given it holds the forward pass' image already.
 // dz: [S][2][m][pad16(f)] 16-bit scratch.  dx, dw_in, dw_out may be null.
-extern "C" int gated_ffn_backward(const void* x, long long ldx, void* x_img, const void* w_in, long long ld_in, void* in_img,
-                                  const void* w_out, long long ld_out, void* out_img, const void* dy, long long ldy,
-                                  void* dy_img, const void* h, const float* z, void* dz, float* partial, void* dx, void* dw_in, void* dw_out,
-                                  int m, int d, int f, int n, int act, int dt, cudaStream_t st) {
+struct FfnBackwardCall {
+  const void* x;
+  long long ldx;
+  void* x_img;
+  const void* w_in;
+  long long ld_in;
+  void* in_img;
+  const void* w_out;
+  long long ld_out;
+  void* out_img;
+  const void* dy;
+  long long ldy;
+  void* dy_img;
+  const void* h;
+  float* z;
+  void* dz;
+  float* partial;
+  void *dx, *dw_in, *dw_out;
+  long long m, d, f, n, act, dt;
+  cudaStream_t st;
+};
+extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
+  const void *x = c->x, *w_in = c->w_in, *w_out = c->w_out, *dy = c->dy, *h = c->h;
+  void *x_img = c->x_img, *in_img = c->in_img, *out_img = c->out_img, *dy_img = c->dy_img, *dz = c->dz;
+  void *dx = c->dx, *dw_in = c->dw_in, *dw_out = c->dw_out;
+  float *z = c->z, *partial = c->partial;
+  const long long ldx = c->ldx, ld_in = c->ld_in, ld_out = c->ld_out, ldy = c->ldy;
+  const int m = (int)c->m, d = (int)c->d, f = (int)c->f, n = (int)c->n, act = (int)c->act, dt = (int)c->dt;
+  const cudaStream_t st = c->st;
   const FfnShape s = {m, d, f, n, act, dt};
   if (!ffn_shape_ok(s)) return -1;
   const int S = dt == DT_F32 ? 3 : 1;
@@ -1043,7 +1088,7 @@ extern "C" int gated_ffn_backward(const void* x, long long ldx, void* x_img, con
   FfnGemm g = base;
   if (dx != nullptr || dw_in != nullptr) {
     g.M = m; g.N = f; g.k_blocks = ffn_k_blocks(S, n); g.b_mn = 1;
-    g.out = dz; g.ldo = pad16(f); g.vec16 = 1; g.z = const_cast<float*>(z); g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
+    g.out = dz; g.ldo = pad16(f); g.vec16 = 1; g.z = z; g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
     if ((rc = ffn_gemm<FF_DGATE>(S, g, oy, oo, st))) return rc;
   }
   if (dx != nullptr) {

@@ -583,28 +583,51 @@ static int ln_run(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStream_t s
   return -1;
 }
 
-// y = layer_norm(x) w + b; mean / rstd may be null (evaluation)
-extern "C" int layer_norm_forward(const void* x, long long ldx, const void* w, const void* b, void* y, float* mean,
-                                  float* rstd, long long n, int d, float eps, int dt, int w_dt, cudaStream_t st) {
+// The calls take one struct of 8-byte members.
+// y = layer_norm(x) w + b; stats: mean [n] and 1 / sqrt(var + eps) [n], or null (evaluation)
+struct LnForwardCall {
+  const void* x;
+  long long ldx;
+  const void *w, *b;
+  void* y;
+  float* stats;
+  long long n, d, dt, w_dt;
+  double eps;
+  cudaStream_t stream;
+};
+extern "C" int layer_norm_forward(const LnForwardCall* c) {
   LnArgs a = {};
-  a.x = x; a.w = w; a.b = b; a.y = y; a.mean = mean; a.rstd = rstd; a.n = n; a.ldx = ldx; a.d = d; a.eps = eps; a.w_dt = w_dt;
+  a.x = c->x; a.w = c->w; a.b = c->b; a.y = c->y; a.n = c->n; a.ldx = c->ldx; a.d = (int)c->d; a.eps = (float)c->eps;
+  a.w_dt = (int)c->w_dt;
+  a.mean = c->stats;
+  a.rstd = c->stats != nullptr ? c->stats + c->n : nullptr;
   int blocks = 0;
-  return ln_run(a, dt, false, &blocks, st);
+  return ln_run(a, (int)c->dt, false, &blocks, c->stream);
 }
 
 // dx (may be null) and dw, db (may be null; partial: layer_norm_partial_floats(d) floats of scratch, or null without both)
-extern "C" int layer_norm_backward(const void* x, long long ldx, const void* dy, long long lddy, const void* w,
-                                   const float* mean, const float* rstd, void* dx, void* dw, void* db, float* partial,
-                                   long long n, int d, int dt, int w_dt, cudaStream_t st) {
-  if ((dw != nullptr || db != nullptr) != (partial != nullptr)) return -1;
+struct LnBackwardCall {
+  const void* x;
+  long long ldx;
+  const void* dy;
+  long long lddy;
+  const void* w;
+  float* stats;
+  void *dx, *dw, *db;
+  float* partial;
+  long long n, d, dt, w_dt;
+  cudaStream_t stream;
+};
+extern "C" int layer_norm_backward(const LnBackwardCall* c) {
+  if ((c->dw != nullptr || c->db != nullptr) != (c->partial != nullptr)) return -1;
   LnArgs a = {};
-  a.x = x; a.dy = dy; a.lddy = lddy; a.w = w; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
-  a.dx = dx; a.partial = partial; a.n = n; a.ldx = ldx; a.d = d; a.w_dt = w_dt;
+  a.x = c->x; a.dy = c->dy; a.lddy = c->lddy; a.w = c->w; a.mean = c->stats; a.rstd = c->stats + c->n;
+  a.dx = c->dx; a.partial = c->partial; a.n = c->n; a.ldx = c->ldx; a.d = (int)c->d; a.w_dt = (int)c->w_dt;
   int blocks = 0;
-  int rc = ln_run(a, dt, true, &blocks, st);
-  if (rc || partial == nullptr) return rc;
-  return (int)launch_k(ln_reduce_kernel, dim3((unsigned)((2LL * d + 31) / 32)), dim3(1024), 0, st, (const float*)partial,
-                       blocks, d, dw, db, w_dt);
+  const int rc = ln_run(a, (int)c->dt, true, &blocks, c->stream);
+  if (rc || c->partial == nullptr) return rc;
+  return (int)launch_k(ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, c->stream,
+                       (const float*)c->partial, blocks, a.d, c->dw, c->db, a.w_dt);
 }
 
 // 0, or 1 after a bounded wait of the backward kernel on the current device ran out (synchronises)

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, Structure, c_float, c_int, c_int32, c_longlong, c_uint32, c_void_p
 
 _LIB = None
@@ -228,3 +229,35 @@ def on_device(device, fn, *args):
         return fn(*args)
     with torch.cuda.device(device):
         return fn(*args)
+
+
+_PACKED = {}
+
+
+def packed(name: str, fmt: str):
+    """The entry point ``name``, which takes one pointer to a struct of 8-byte members (``fmt``: ``q`` pointers and integers,
+    ``d`` floating numbers), as a function of the members that returns the error code.  One ``struct.pack`` costs a fraction of
+    converting twenty arguments one by one, which would be a third of the host time of a small call."""
+    call = _PACKED.get(name)
+    if call is None:
+        fn = getattr(load(), name)
+        fn.argtypes, fn.restype = [ctypes.c_char_p], c_int
+        pack = struct.Struct("=" + fmt).pack
+        call = _PACKED[name] = lambda *members: fn(pack(*members))
+    return call
+
+
+def raw_stream(device) -> int:
+    """``cudaStream_t`` of the current stream of ``device`` as an integer."""
+    import torch
+
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(device.index) if get is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def no_second_derivative(what: str):
+    """Raised in a backward pass that is itself being recorded (``create_graph=True``)."""
+    import torch
+
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: the backward kernels have no derivative (create_graph=True)")

@@ -9,22 +9,10 @@ draws one from PyTorch's generator (``torch.manual_seed``, checkpointed generato
 the library's dropout).  Layers that share a key give different ``site`` numbers."""
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from .norm import DT
-
-
-def _declare():
-    lib = _lib.load()
-    if not getattr(lib, "_dropout_declared", False):
-        vp, i, ll, u = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_uint
-        lib.dropout_apply.argtypes = [vp, vp, vp, ll, vp, u, u, i, vp]
-        lib.dropout_apply.restype = i
-        lib._dropout_declared = True
-    return lib
+from .norm import DT, ptr
 
 
 def new_key(device) -> torch.Tensor:
@@ -38,13 +26,13 @@ def drop_steps(p: float) -> int:
 
 
 def _apply(x, residual, key, drop, site):
-    x = x.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if x.numel():
-        lib = _declare()
-        _lib.check(lib.dropout_apply(x.data_ptr(), residual.data_ptr() if residual is not None else 0, y.data_ptr(),
-                                     x.numel(), key.data_ptr(), site, drop, DT[x.dtype], _lib.stream_ptr()),
-                   "dropout_apply")
+    if not x.is_contiguous():
+        x = x.contiguous()
+    y = torch.empty_like(x)
+    n = x.numel()
+    if n:
+        _lib.check(_lib.packed("dropout_apply", "9q")(x.data_ptr(), ptr(residual), y.data_ptr(), n, key.data_ptr(), site, drop,
+                                                      DT[x.dtype], _lib.raw_stream(x.device)), "dropout_apply")
         _lib.count(1)
     return y
 
@@ -59,7 +47,10 @@ class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (key,) = ctx.saved_tensors
-        dx = _DropoutFn.apply(dy, None, key, ctx.drop, ctx.site) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            # the gradient's gradient is the same function again
+            dx = (_DropoutFn.apply if torch.is_grad_enabled() else _apply)(dy, None, key, ctx.drop, ctx.site)
         return dx, dy if ctx.has_residual else None, None, None, None
 
 

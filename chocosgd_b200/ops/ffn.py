@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .norm import DT, rows_of
+from .norm import DT, ptr, rows_of
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 
@@ -20,10 +20,8 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 def _declare():
     lib = _lib.load()
     if not getattr(lib, "_ffn_declared", False):
-        vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        lib.gated_ffn_forward.argtypes = [vp, ll, vp] * 3 + [vp] * 4 + [i] * 7 + [vp]
-        lib.gated_ffn_backward.argtypes = [vp, ll, vp] * 4 + [vp] * 7 + [i] * 6 + [vp]
-        lib.gated_ffn_forward.restype = lib.gated_ffn_backward.restype = lib.gated_ffn_last_error.restype = i
+        i, ll = ctypes.c_int, ctypes.c_longlong
+        lib.gated_ffn_last_error.restype = i
         lib.gated_ffn_few_tokens.argtypes = [i]
         lib.gated_ffn_few_tokens.restype = i
         lib.gated_ffn_partial_floats.argtypes = [i] * 6
@@ -71,7 +69,7 @@ class _Layout:
 
 
 def _at(base, offset):
-    return None if offset is None else base + offset
+    return 0 if offset is None else base + offset
 
 
 class _GatedFfnFn(torch.autograd.Function):
@@ -95,9 +93,10 @@ class _GatedFfnFn(torch.autograd.Function):
         buf = torch.empty(lay.size, dtype=torch.uint8, device=x.device)
         if m:
             b = buf.data_ptr()
-            rc = lib.gated_ffn_forward(x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
-                                       wo.data_ptr(), wo.stride(0), _at(b, img[2]), b + h, _at(b, z), _at(b, partial),
-                                       y.data_ptr(), m, d, f, n, act, dt, int(few), _lib.stream_ptr())
+            rc = _lib.packed("gated_ffn_forward", "21q")(
+                x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
+                wo.data_ptr(), wo.stride(0), _at(b, img[2]), b + h, _at(b, z), _at(b, partial),
+                y.data_ptr(), m, d, f, n, act, dt, int(few), _lib.raw_stream(x2.device))
             if rc:
                 raise RuntimeError(f"gated_ffn_forward failed with code {rc}")
             _lib.count(2 + int(any(i is not None for i in img)) + int(partial is not None))
@@ -107,8 +106,8 @@ class _GatedFfnFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _lib.no_second_derivative("gated_ffn")
         lib = _declare()
         x2, wi, wo, buf = ctx.saved_tensors
         img, h, z = ctx.layout
@@ -126,10 +125,11 @@ class _GatedFfnFn(torch.autograd.Function):
             partial = lay.scratch(lib.gated_ffn_partial_floats(m, d, f, n, DT[x2.dtype], 1))
             scratch = torch.empty(lay.size, dtype=torch.uint8, device=x2.device)
             b, s = buf.data_ptr(), scratch.data_ptr()
-            rc = lib.gated_ffn_backward(x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
-                                        wo.data_ptr(), wo.stride(0), _at(b, img[2]), dy2.data_ptr(), dy2.stride(0),
-                                        _at(s, dy_img), b + h, b + z, s + dz, _at(s, partial), _lib.ptr(dx), _lib.ptr(dwi),
-                                        _lib.ptr(dwo), m, d, f, n, ctx.act, DT[x2.dtype], _lib.stream_ptr())
+            rc = _lib.packed("gated_ffn_backward", "26q")(
+                x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
+                wo.data_ptr(), wo.stride(0), _at(b, img[2]), dy2.data_ptr(), dy2.stride(0),
+                _at(s, dy_img), b + h, b + z, s + dz, _at(s, partial), ptr(dx), ptr(dwi),
+                ptr(dwo), m, d, f, n, ctx.act, DT[x2.dtype], _lib.raw_stream(x2.device))
             if rc:
                 raise RuntimeError(f"gated_ffn_backward failed with code {rc}")
             _lib.count(int(need[0] or need[1]) + sum(need[:3]) + int(dy_img is not None))

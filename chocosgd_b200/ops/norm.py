@@ -15,17 +15,20 @@ from . import _lib
 DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _declare():
+def _partial_floats(d: int) -> int:
     lib = _lib.load()
     if not getattr(lib, "_ln_declared", False):
-        vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        lib.layer_norm_forward.argtypes = [vp, ll, vp, vp, vp, vp, vp, ll, i, ctypes.c_float, i, i, vp]
-        lib.layer_norm_backward.argtypes = [vp, ll, vp, ll, vp, vp, vp, vp, vp, vp, vp, ll, i, i, i, vp]
-        lib.layer_norm_partial_floats.argtypes = [i]
-        lib.layer_norm_partial_floats.restype = ll
-        lib.layer_norm_forward.restype = lib.layer_norm_backward.restype = i
+        lib.layer_norm_partial_floats.argtypes = [ctypes.c_int]
+        lib.layer_norm_partial_floats.restype = ctypes.c_longlong
+        lib.layer_norm_last_error.restype = ctypes.c_int
         lib._ln_declared = True
-    return lib
+    return lib.layer_norm_partial_floats(d)
+
+
+def last_error() -> int:
+    """Non-zero after a bounded wait of the backward kernel on the current device ran out (synchronises)."""
+    _partial_floats(1)
+    return _lib.load().layer_norm_last_error()
 
 
 def rows_of(x: torch.Tensor) -> torch.Tensor:
@@ -34,48 +37,47 @@ def rows_of(x: torch.Tensor) -> torch.Tensor:
     return x2 if x2.stride(1) == 1 and x2.stride(0) >= x2.shape[1] else x2.contiguous()
 
 
+def ptr(t) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        lib = _declare()
         x2 = rows_of(x)
         n, d = x2.shape
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dev = x.device
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
         p = weight if weight is not None else bias
-        ctx.p_dtype = p.dtype if p is not None else x.dtype
-        train = any(ctx.needs_input_grad)
-        stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if train else None
+        ctx.p_dtype = p_dtype = p.dtype if p is not None else x.dtype
+        stats = torch.empty(2 * n, dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
         if n:
-            sp = stats.data_ptr() if train else 0
-            _lib.check(lib.layer_norm_forward(x2.data_ptr(), x2.stride(0), _lib.ptr(weight), _lib.ptr(bias), y.data_ptr(),
-                                              sp, sp + 4 * n if train else 0, n, d, eps, DT[x.dtype], DT[ctx.p_dtype],
-                                              _lib.stream_ptr()), "layer_norm_forward")
+            _lib.check(_lib.packed("layer_norm_forward", "10qdq")(
+                x2.data_ptr(), x2.stride(0), ptr(weight), ptr(bias), y.data_ptr(), ptr(stats), n, d, DT[x.dtype], DT[p_dtype], eps,
+                _lib.raw_stream(dev)), "layer_norm_forward")
             _lib.count(1)
-        if train:
+        if stats is not None:
             ctx.save_for_backward(x2, weight, stats)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        lib = _declare()
+        _lib.no_second_derivative("layer_norm")
         x2, weight, stats = ctx.saved_tensors
         n, d = x2.shape
-        dev, need = x2.device, ctx.needs_input_grad
-        dx = torch.empty(dy.shape, dtype=x2.dtype, device=dev) if need[0] else None
+        dev, (need_x, need_w, need_b, _) = x2.device, ctx.needs_input_grad
+        dx = torch.empty_like(dy, memory_format=torch.contiguous_format) if need_x else None
         make = torch.empty if n else torch.zeros
-        dw = make(d, dtype=ctx.p_dtype, device=dev) if need[1] else None
-        db = make(d, dtype=ctx.p_dtype, device=dev) if need[2] else None
+        dw = make(d, dtype=ctx.p_dtype, device=dev) if need_w else None
+        db = make(d, dtype=ctx.p_dtype, device=dev) if need_b else None
         if n:
             dy2 = rows_of(dy)
             partial = None
-            if need[1] or need[2]:
-                partial = torch.empty(lib.layer_norm_partial_floats(d), dtype=torch.float32, device=dev)
-            sp = stats.data_ptr()
-            _lib.check(lib.layer_norm_backward(x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), _lib.ptr(weight),
-                                               sp, sp + 4 * n, _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(partial),
-                                               n, d, DT[x2.dtype], DT[ctx.p_dtype], _lib.stream_ptr()),
-                       "layer_norm_backward")
+            if need_w or need_b:
+                partial = torch.empty(_partial_floats(d), dtype=torch.float32, device=dev)
+            _lib.check(_lib.packed("layer_norm_backward", "15q")(
+                x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), ptr(weight), stats.data_ptr(), ptr(dx), ptr(dw),
+                ptr(db), ptr(partial), n, d, DT[x2.dtype], DT[ctx.p_dtype], _lib.raw_stream(dev)), "layer_norm_backward")
             _lib.count(2 if partial is not None else 1)
         return dx, dw, db, None
 
