@@ -200,6 +200,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--rnn_use_pretrained_emb", type=str2bool, default=True)
     p.add_argument("--rnn_tie_weights", type=str2bool, default=True)
     p.add_argument("--rnn_weight_norm", type=str2bool, default=False)
+    p.add_argument("--rnn_n_ffn", default=0, type=int,
+                   help="hidden width of a gated feed-forward block between the LSTM stack and the decoder (0: none)")
+    p.add_argument("--rnn_ffn_act", default="silu", choices=("silu", "gelu", "relu", "sigmoid"))
     p.add_argument("--mlp_num_layers", default=2, type=int)
     p.add_argument("--mlp_hidden_size", default=500, type=int)
 
@@ -275,6 +278,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--use_cuda_graph", default=True, type=str2bool)
     p.add_argument("--channels_last", default=True, type=str2bool,
                    help="keep 4-d activations and convolution weights in NHWC / KRSC memory order on CUDA")
+    p.add_argument("--counter_dropout", default=False, type=str2bool,
+                   help="dropout masks on CUDA from a counter-based generator instead of the library's: recomputed in the "
+                   "backward pass, never stored (other masks from the same seed)")
     p.add_argument("--native_layers", default="auto", choices=("auto", "all", "off", "bn", "conv"),
                    help="layers routed to the hand-written sm_100a kernels on CUDA: auto = batch-norm + 3x3 "
                    "convolution fwd/dgrad/wgrad, all = auto + linear + LSTM cell, "
@@ -356,6 +362,8 @@ def get_args(argv: Optional[Sequence[str]] = None, strict: bool = False) -> Conf
 def validate(conf: Config) -> None:
     """Fail fast on inconsistent combinations (the convex code does this with asserts,
     ``convex_code/parameters.py:34-71``; the deep-learning code does not)."""
+    if getattr(conf, "rnn_n_ffn", 0) < 0:
+        raise ValueError(f"--rnn_n_ffn is a width, got {conf.rnn_n_ffn}")
     needs_op = ("parallel_choco", "parallel_choco_v", "dcd_psgd", "ecd_psgd", "deep_squeeze", "dgc")
     if conf.optimizer in needs_op and conf.comm_op is None:
         raise ValueError(f"--optimizer {conf.optimizer} needs --comm_op")

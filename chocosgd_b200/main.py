@@ -71,6 +71,8 @@ def main(conf):
         from .ops import nn as native_nn
 
         native_nn.configure_native(getattr(conf, "native_layers", "auto"))
+        if getattr(conf, "counter_dropout", False):
+            native_nn.set_native(True, which=("dropout",))
     data_loader = define_dataset(conf, graph, run, device=device)
     model = define_model(conf, graph, data_loader=data_loader, device=device)
     optimizer = define_optimizer(conf, model, graph)

@@ -41,6 +41,8 @@ def define_nlp_model(conf, n_tokens, emb_size=None, pretrained=None):
         tie_weights=conf.rnn_tie_weights,
         dropout=conf.drop_rate,
         weight_norm=conf.rnn_weight_norm,
+        nffn=getattr(conf, "rnn_n_ffn", 0),
+        ffn_act=getattr(conf, "rnn_ffn_act", "silu"),
     )
     if pretrained is not None:
         model.encoder.weight.data.copy_(pretrained)

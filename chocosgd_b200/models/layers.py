@@ -19,7 +19,9 @@ Linear = native_nn.Linear
 ReLU = nn.ReLU
 MaxPool2d = native_nn.MaxPool2d
 AvgPool2d = nn.AvgPool2d
-Dropout = nn.Dropout
+Dropout = native_nn.Dropout
+LayerNorm = native_nn.LayerNorm
+GatedFeedForward = native_nn.GatedFeedForward
 Embedding = native_nn.Embedding
 LSTM = native_nn.LSTM
 
@@ -78,6 +80,19 @@ def he_init(module: nn.Module, zero_linear_bias: bool = False):
             m.bias.data.zero_()
         elif zero_linear_bias and isinstance(m, nn.Linear) and m.bias is not None:
             m.bias.data.zero_()
+
+
+class FeedForwardBlock(nn.Module):
+    """Pre-norm residual block ``x + dropout(ffn(norm(x)))`` with a gated feed-forward layer."""
+
+    def __init__(self, dim, hidden, act="silu", dropout=0.0):
+        super().__init__()
+        self.norm = LayerNorm(dim)
+        self.ffn = GatedFeedForward(dim, hidden, act)
+        self.drop = Dropout(dropout, counter=True)
+
+    def forward(self, x):
+        return self.drop(self.ffn(self.norm(x)).to(x.dtype), x)
 
 
 def num_classes_of(dataset: str) -> int:

@@ -143,6 +143,16 @@ def lstm_supported(m, x) -> bool:
             and x.dtype == torch.float32 and x.is_cuda)
 
 
+def _layer_dropout(x, p):
+    from . import nn as native_nn
+
+    if native_nn.native_enabled("dropout"):
+        from .dropout import dropout, new_key
+
+        return dropout(x, p, new_key(x.device))
+    return F.dropout(x, p=p, training=True)
+
+
 def lstm_native(m, x, hx=None):
     T, B, _ = x.shape
     L, H = m.num_layers, m.hidden_size
@@ -158,5 +168,5 @@ def lstm_native(m, x, hx=None):
         hn.append(h)
         cn.append(c)
         if m.dropout > 0 and m.training and l < L - 1:
-            out = F.dropout(out, p=m.dropout, training=True)
+            out = _layer_dropout(out, m.dropout)
     return out, (torch.stack(hn), torch.stack(cn))

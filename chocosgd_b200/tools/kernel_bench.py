@@ -11,6 +11,8 @@
     python -m chocosgd_b200.tools.kernel_bench --case conv_s2 --batch 128 --hw 32 --channels 16    # strided forward + input gradient
     python -m chocosgd_b200.tools.kernel_bench --case maxpool --batch 64 --hw 112 --channels 64
     python -m chocosgd_b200.tools.kernel_bench --case stem --batch 64 --hw 224                     # 7x7 / 2 bf16 stem, forward and wgrad
+    python -m chocosgd_b200.tools.kernel_bench --case norm --m 16384 --n 4096 --dtype bf16         # layer norm, also --case dropout
+    python -m chocosgd_b200.tools.kernel_bench --case ffn --m 4096 --k 1024 --n 4096 --dtype bf16  # m tokens, width k, hidden n
 """
 from __future__ import annotations
 
@@ -41,7 +43,8 @@ def timed(fn, iters):
 def main(argv=None):
     p = argparse.ArgumentParser()
     p.add_argument("--case", required=True, choices=("sign", "topk", "qsgd", "randk", "gemm", "conv", "wgrad", "bn", "bn16", "wgrad_gen",
-                                                    "conv_s2", "maxpool", "stem"))
+                                                    "conv_s2", "maxpool", "stem", "norm", "dropout", "ffn"))
+    p.add_argument("--dtype", default="bf16", choices=("fp32", "bf16", "fp16"))
     p.add_argument("--ks", type=int, default=3)
     p.add_argument("--stride", type=int, default=1)
     p.add_argument("--elements", type=int, default=64 * 1024 * 1024)
@@ -73,6 +76,36 @@ def main(argv=None):
         eng.flush()
         out.update(elements=a.elements, ms=ms, bytes_per_elem_model=32 + 3 / 8.0,
                    achieved_GBps=(32 + 3 / 8.0) * a.elements / ms / 1e6, kernels=eng.launches_per_step)
+    elif a.case in ("norm", "dropout", "ffn"):
+        dt = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}[a.dtype]
+        if a.case == "ffn":
+            from ..ops.ffn import gated_ffn
+
+            x = torch.randn(a.m, a.k, device=dev).to(dt).requires_grad_()
+            leaves = (x, (torch.randn(2 * a.n, a.k, device=dev) * a.k ** -0.5).to(dt).requires_grad_(),
+                      (torch.randn(a.k, a.n, device=dev) * a.n ** -0.5).to(dt).requires_grad_())
+            fwd = lambda: gated_ffn(*leaves)  # noqa: E731
+        else:
+            x = torch.randn(a.m, a.n, device=dev).to(dt).requires_grad_()
+            if a.case == "norm":
+                from ..ops.norm import layer_norm
+
+                leaves = (x, torch.ones(a.n, device=dev, dtype=dt).requires_grad_(), torch.zeros(a.n, device=dev, dtype=dt).requires_grad_())
+                fwd = lambda: layer_norm(*leaves)  # noqa: E731
+            else:
+                from ..ops.dropout import dropout, new_key
+
+                key, leaves = new_key(dev), (x,)
+                fwd = lambda: dropout(x, 0.1, key)  # noqa: E731
+        y = fwd()
+        dy = torch.randn_like(y)
+        ms_f = timed(lambda: fwd(), a.iters)
+        ms_b = timed(lambda: torch.autograd.grad(y, leaves, dy, retain_graph=True), a.iters)
+        out.update(m=a.m, n=a.n, k=a.k, dtype=a.dtype, forward_ms=ms_f, backward_ms=ms_b)
+        if a.case == "ffn":
+            out["tflops"] = 18e-9 * a.m * a.n * a.k / (ms_f + ms_b)
+        else:
+            out["gbs"] = (4 if a.case == "dropout" else 5) * x.numel() * x.element_size() * 1e-6 / (ms_f + ms_b)
     elif a.case == "gemm":
         from ..ops.gemm import gemm, last_error
 

@@ -19,7 +19,8 @@ def main(argv=None):
     p.add_argument("--steps", type=int, default=50)
     p.add_argument("--warmup", type=int, default=5)
     p.add_argument("--no_graph", action="store_true")
-    p.add_argument("--native", default="off", help="comma list of native layer kinds (ce, lstm, linear) or off")
+    p.add_argument("--native", default="off", help="comma list of native layer kinds (ce, lstm, linear, norm, ffn, dropout) or off")
+    p.add_argument("--ffn", type=int, default=0, help="hidden width of a gated feed-forward block behind the LSTM stack")
     p.add_argument("--tf32_matmul", action="store_true",
                    help="let the library run the fp32 decoder / embedding GEMMs on TF32 tensor cores (PyTorch keeps "
                         "them on fp32 FMA units by default, which is 3.1 of the 6.2 ms step; the LSTM's own GEMMs "
@@ -45,7 +46,7 @@ def main(argv=None):
                      "--quantize_level", "4", "--is_biased", "True", "--graph_topology", "ring",
                      "--n_mpi_process", str(world), "--lr", "2.5", "--momentum_factor", "0.0", "--weight_decay", "0",
                      "--consensus_stepsize", "0.3", "--rnn_n_hidden", "650", "--rnn_n_layers", "2", "--drop_rate", "0.4",
-                     "--rnn_clip", "0.4", "--batch_size", str(B), "--gossip_impl", "fused"])
+                     "--rnn_clip", "0.4", "--batch_size", str(B), "--gossip_impl", "fused", "--rnn_n_ffn", str(a.ffn)])
     graph = Graph("ring", world, rank)
     torch.manual_seed(6)
     if a.native != "off":
@@ -81,7 +82,7 @@ def main(argv=None):
     opt.engine.check()
     if rank == 0:
         print(json.dumps({"bench": "lstm_lm", "n_gpus": world, "tokens_per_s": B * T * world * a.steps / (ms * 1e-3),
-                          "ms_per_step": ms / a.steps, "loss": float(loss), "graph": step.use_graph, "native": a.native, "tf32_matmul": bool(a.tf32_matmul),
+                          "ms_per_step": ms / a.steps, "loss": float(loss), "graph": step.use_graph, "native": a.native, "ffn": a.ffn, "tf32_matmul": bool(a.tf32_matmul),
                           "kernels_per_step": opt.engine.launches_per_step, "comm_op": "quantize_qsgd 4 bit",
                           "params": sum(p.numel() for p in model.parameters())}))
     if world > 1:
