@@ -107,7 +107,119 @@ __device__ __forceinline__ int ln_slot(int vectors, int c) {      // where eleme
   return V >= 4 ? ((c % V / 4) * vectors + c / V) * 4 + c % 4 : c;
 }
 
-// Rows of up to 32 V NV elements per warp.  16384 x 4096 bf16: see the kernel's figures in the launch code.
+#define LN_RING 3        // rows of a group under way (backward)
+#define LN_T16 640       // threads of a block with 16 elements per thread (96 registers)
+
+__device__ __forceinline__ void ln_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// parameters of vector v as pairs
+template <int V>
+__device__ __forceinline__ void ln_get2(const float* s, int vectors, int v, F2 (&out)[V / 2]) {
+#pragma unroll
+  for (int h = 0; h < V / 4; ++h) {
+    const float4 q = reinterpret_cast<const float4*>(s)[h * vectors + v];
+    out[2 * h] = f2(q.x, q.y);
+    out[2 * h + 1] = f2(q.z, q.w);
+  }
+}
+
+// Rows on 16-byte boundaries, four vectors per lane.  A group (one warp up to 1024 16-bit elements) has two rows or more of its
+// own coming into shared memory by bulk copies while it works on a third in registers; the stage is filled again as soon as
+// the registers have it.  Arithmetic in pairs of fp32 numbers: one element at a time the kernel is bound by issue (18 instructions
+// per element; 16384 x 4096 bf16: 85 us, with pairs and 8 vectors per lane 77, with 4 vectors 63; 65536 x 1024: 49).
+template <typename T, int NV>
+__global__ void __launch_bounds__(512, 1) ln_fwd_ring_kernel(LnArgs a, int threads, int groups, int depth) {
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ float4 ln_smem4[];
+  __shared__ float red[16][2][32];
+  __shared__ uint64_t full[16][8];
+  const int vectors = a.d / V, row_bytes = vectors * 16;
+  float *w_s = reinterpret_cast<float*>(ln_smem4), *b_s = w_s + a.d;
+  const int group = threadIdx.x / threads, t = threadIdx.x % threads;
+  uint8_t* mine = reinterpret_cast<uint8_t*>(b_s + a.d) + (long long)group * depth * row_bytes;
+  if (t == 0) {
+    for (int k = 0; k < depth; ++k) mbar_init(&full[group][k], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const long long first = (long long)blockIdx.x * groups + group, stride = (long long)gridDim.x * groups;
+  const auto fill = [&](long long row, int k) {
+    mbar_expect_tx(&full[group][k], row_bytes);
+    ln_bulk(mine + k * row_bytes, x + row * a.ldx, row_bytes, &full[group][k]);
+  };
+  if (t == 0)
+    for (int k = 0; k < depth; ++k)
+      if (first + k * stride < a.n) fill(first + k * stride, k);
+  for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+    w_s[ln_slot<V>(vectors, c)] = ln_param(a.w, a.w_dt, c, 1.f);
+    b_s[ln_slot<V>(vectors, c)] = ln_param(a.b, a.w_dt, c, 0.f);
+  }
+  __syncthreads();
+  const float inv_d = 1.f / (float)a.d;
+  int k = 0;
+  uint32_t phase = 0;
+  for (long long row = first; row < a.n; row += stride) {
+    if (!mbar_wait(&full[group][k], phase)) atomicExch(&g_ln_error, 1);
+    Vec<T, V> r[NV];
+    F2 sum = f2(0.f), more = f2(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      r[j].clear();
+      if (j * threads + t < vectors) r[j].load(reinterpret_cast<const T*>(mine + k * row_bytes) + (j * threads + t) * V);
+#pragma unroll
+      for (int i = 0; i < V / 2; i += 2) {
+        sum = sum + pair_of(r[j], i);
+        more = more + pair_of(r[j], i + 1);
+      }
+    }
+    float s[1] = {f2_sum(sum) + f2_sum(more)};
+    ln_group_sum<1>(s, red[group][0], group, t, threads);      // every thread has the row in registers
+    if (t == 0 && row + depth * stride < a.n) fill(row + depth * stride, k);
+    const float mu = s[0] * inv_d;
+    sum = more = f2(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) opaque(r[j].raw);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (j * threads + t < vectors) {
+#pragma unroll
+        for (int i = 0; i < V / 2; i += 2) {
+          const F2 p = pair_of(r[j], i) + f2(-mu), q = pair_of(r[j], i + 1) + f2(-mu);
+          sum = f2_fma(p, p, sum);
+          more = f2_fma(q, q, more);
+        }
+      }
+    s[0] = f2_sum(sum) + f2_sum(more);
+    ln_group_sum<1>(s, red[group][1], group, t, threads);
+    const float rs = 1.f / sqrtf(fmaf(s[0], inv_d, a.eps));
+    const F2 rs2 = f2(rs), off = f2(-mu * rs);
+    T* y = reinterpret_cast<T*>(a.y) + row * a.d;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) opaque(r[j].raw);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (j * threads + t < vectors) {
+        F2 w[V / 2], b[V / 2];
+        ln_get2<V>(w_s, vectors, j * threads + t, w);
+        ln_get2<V>(b_s, vectors, j * threads + t, b);
+        F2 o[V / 2];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) o[i] = f2_fma(f2_fma(pair_of(r[j], i), rs2, off), w[i], b[i]);
+        store_pairs(y + (j * threads + t) * V, o);
+      }
+    if (t == 0 && a.mean != nullptr) {
+      a.mean[row] = mu;
+      a.rstd[row] = rs;
+    }
+    if (++k == depth) { k = 0; phase ^= 1; }
+  }
+}
+
+// Other rows, and few rows: up to 32 V NV elements per warp, in registers.
 template <typename T, int V, int NV>
 __global__ void __launch_bounds__(256, NV >= 16 ? 2 : 4) ln_fwd_kernel(LnArgs a, int threads, int groups) {
   extern __shared__ float4 ln_smem4[];
@@ -177,18 +289,11 @@ __global__ void __launch_bounds__(256, NV >= 16 ? 2 : 4) ln_fwd_kernel(LnArgs a,
   }
 }
 
-#define LN_RING 3        // rows of a group under way
-
-__device__ __forceinline__ void ln_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-
 // Rows on 16-byte boundaries.  x and dy of a row lie in a stage of the group's ring and are read there twice, before and after
-// the row's two sums are known; registers hold only the sums of dw and db (32 at 16 elements per thread, 1024 threads).  The stage
+// the row's two sums are known; registers hold only the sums of dw and db.  The stage
 // of the row before is filled again behind the barrier of the row's sums: by then every thread is done with it.
 template <typename T, int E>
-__global__ void __launch_bounds__(1024, 1) ln_bwd_ring_kernel(LnArgs a, int threads, int groups) {
+__global__ void __launch_bounds__(E == 8 ? 1024 : LN_T16, 1) ln_bwd_ring_kernel(LnArgs a, int threads, int groups) {
   constexpr int V = 16 / sizeof(T), NV = E / V;
   extern __shared__ float4 ln_smem4[];
   __shared__ float red[16][2][64];
@@ -216,9 +321,9 @@ __global__ void __launch_bounds__(1024, 1) ln_bwd_ring_kernel(LnArgs a, int thre
   if (t == 0)
     for (int k = 0; k < LN_RING - 1; ++k)
       if (first + k * stride < a.n) fill(first + k * stride, k);
-  float dw[E], db[E];
+  F2 dw[E / 2], db[E / 2];
 #pragma unroll
-  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
+  for (int e = 0; e < E / 2; ++e) dw[e] = db[e] = f2(0.f);
   const float inv_d = 1.f / (float)a.d;
   int turn = 0, k = 0;
   uint32_t phase = 0;
@@ -231,7 +336,8 @@ __global__ void __launch_bounds__(1024, 1) ln_bwd_ring_kernel(LnArgs a, int thre
     }
     if (!mbar_wait(&full[group][k], phase)) atomicExch(&g_ln_error, 1);
     const uint4 *xs = reinterpret_cast<const uint4*>(mine + k * 2 * row_bytes), *gs = xs + vectors;
-    float s[2] = {0.f, 0.f};
+    const F2 rs2 = f2(rs), off = f2(-mu * rs);
+    F2 s0 = f2(0.f), s1 = f2(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int v = j * threads + t;
@@ -239,39 +345,40 @@ __global__ void __launch_bounds__(1024, 1) ln_bwd_ring_kernel(LnArgs a, int thre
         Vec<T, V> px, pg;
         px.load(reinterpret_cast<const T*>(xs + v));
         pg.load(reinterpret_cast<const T*>(gs + v));
-        float w[V];
-        ln_get<V>(w_s, vectors, v, w);
+        F2 w[V / 2];
+        ln_get2<V>(w_s, vectors, v, w);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float z = (to_f(px.e[e]) - mu) * rs, g = to_f(pg.e[e]), gw = g * w[e];
-          dw[j * V + e] = fmaf(g, z, dw[j * V + e]);
-          db[j * V + e] += g;
-          s[0] += gw;
-          s[1] = fmaf(gw, z, s[1]);
+        for (int i = 0; i < V / 2; ++i) {
+          const F2 z = f2_fma(pair_of(px, i), rs2, off), g = pair_of(pg, i), gw = g * w[i];
+          dw[j * V / 2 + i] = f2_fma(g, z, dw[j * V / 2 + i]);
+          db[j * V / 2 + i] = db[j * V / 2 + i] + g;
+          s0 = s0 + gw;
+          s1 = f2_fma(gw, z, s1);
         }
       }
     }
+    float s[2] = {f2_sum(s0), f2_sum(s1)};
     ln_group_sum<2>(s, red[group][turn], group, t, threads);
     if (threads == 32) __syncwarp();
     if (t == 0 && row + (LN_RING - 1) * stride < a.n) fill(row + (LN_RING - 1) * stride, (k + LN_RING - 1) % LN_RING);
     if (a.dx != nullptr) {
-      const float mg = s[0] * inv_d, mgz = s[1] * inv_d;
+      const F2 mg = f2(-s[0] * inv_d), mgz = f2(-s[1] * inv_d);
       T* dx = reinterpret_cast<T*>(a.dx) + row * a.d;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int v = j * threads + t;
         if (v < vectors) {
-          Vec<T, V> px, pg, o;
+          Vec<T, V> px, pg;
           px.load(reinterpret_cast<const T*>(xs + v));
           pg.load(reinterpret_cast<const T*>(gs + v));
-          float w[V];
-          ln_get<V>(w_s, vectors, v, w);
+          F2 w[V / 2], o[V / 2];
+          ln_get2<V>(w_s, vectors, v, w);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float z = (to_f(px.e[e]) - mu) * rs;
-            o.e[e] = from_f<T>(rs * (fmaf(to_f(pg.e[e]), w[e], -mg) - z * mgz));
+          for (int i = 0; i < V / 2; ++i) {
+            const F2 z = f2_fma(pair_of(px, i), rs2, off);
+            o[i] = f2_fma(z, mgz, f2_fma(pair_of(pg, i), w[i], mg)) * rs2;
           }
-          o.store(dx + v * V);
+          store_pairs(dx + v * V, o);
         }
       }
     }
@@ -289,9 +396,12 @@ __global__ void __launch_bounds__(1024, 1) ln_bwd_ring_kernel(LnArgs a, int thre
       const int v = j * threads + t;
       if (v < vectors) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          acc_s[v * V + e] += dw[j * V + e];
-          acc_s[a.d + v * V + e] += db[j * V + e];
+        for (int i = 0; i < V / 2; ++i) {
+          const float2 pw = f2_get(dw[j * V / 2 + i]), pb = f2_get(db[j * V / 2 + i]);
+          acc_s[v * V + 2 * i] += pw.x;
+          acc_s[v * V + 2 * i + 1] += pw.y;
+          acc_s[a.d + v * V + 2 * i] += pb.x;
+          acc_s[a.d + v * V + 2 * i + 1] += pb.y;
         }
       }
     }
@@ -502,6 +612,34 @@ static int ln_launch_fwd(const LnArgs& a, cudaStream_t st) {
   }
   return (int)launch_k(kernel, dim3((unsigned)blocks), dim3((unsigned)(threads * groups)), (size_t)smem, st, a, threads, groups);
 }
+template <typename T, int NV>
+static int ln_launch_fwd_ring(const LnArgs& a, cudaStream_t st, bool* done) {
+  constexpr int V = 16 / sizeof(T);
+  const int threads = 32 * ((a.d + 32 * V * NV - 1) / (32 * V * NV)), row_bytes = a.d * (int)sizeof(T);
+  if (threads > 512) return 0;
+  int groups = 512 / threads;
+  if (groups > 15 && threads > 32) groups = 15;
+  int depth = (int)((215 * 1024 - 8LL * a.d) / ((long long)groups * row_bytes));
+  if (depth > 8) depth = 8;
+  if (depth < 2) return 0;
+  if ((long long)groups * depth * row_bytes > 96 * 1024 && depth > 3) depth = 3;      // about what covers the latency
+  *done = true;
+  const int smem = 8 * a.d + groups * depth * row_bytes;
+  void (*kernel)(LnArgs, int, int, int) = ln_fwd_ring_kernel<T, NV>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return (int)e;
+  const long long blocks = (a.n + groups - 1) / groups, most = sm_count();
+  return (int)launch_k(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3((unsigned)(threads * groups)), (size_t)smem, st,
+                       a, threads, groups, depth);
+}
+// The ring: rows of at least 2 KB on 16-byte boundaries, enough of them for sixteen warps on every SM, room for two per group.
+template <typename T>
+static int ln_fwd_ring(const LnArgs& a, cudaStream_t st, bool* done) {
+  *done = false;
+  if (a.n < 16LL * sm_count() || a.d * (long long)sizeof(T) < 2048) return 0;
+  return ln_launch_fwd_ring<T, 4>(a, st, done);
+}
+
 // Vectors per lane: 16 when there are rows for eight warps on every SM (a row per warp needs no block barrier), and where the
 // row would not fit otherwise; else 4 or 2, so that more warps share a row's latency.
 template <typename T, int V>
@@ -519,7 +657,7 @@ static int ln_launch_bwd(const LnArgs& a, int* blocks, cudaStream_t st) {
   const int threads = ln_threads(a.d, E);
   if (threads > 1024) return -1;
   const long long per_sm = (a.n + sm_count() - 1) / sm_count();
-  long long groups = 1024 / threads;
+  long long groups = (RING && E == 16 ? LN_T16 : 1024) / threads;
   if (groups > 15 && threads > 32) groups = 15;     // named barriers 1 .. 15
   if (RING && groups > 16) groups = 16;
   if (groups > per_sm) groups = per_sm;
@@ -560,15 +698,20 @@ static int ln_dispatch(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStrea
   const int v = ln_vec(a, dt, bwd);
   constexpr int W = 16 / sizeof(T);
   if (!bwd) {
-    if (v == W) return ln_fwd<T, W>(a, st);
+    if (v == W) {
+      bool done;
+      const int rc = ln_fwd_ring<T>(a, st, &done);
+      return done || rc ? rc : ln_fwd<T, W>(a, st);
+    }
     if (v == 2) return ln_fwd<T, 2>(a, st);
     return ln_fwd<T, 1>(a, st);
   }
-  // 16 elements per thread for 16-bit rows (two vectors; the sums' shuffles weigh half), 8 for fp32; the ring where its three rows fit
+  // The ring where its three rows fit, with 8 elements per thread, for 16-bit rows from 1024 on (and for rows above 8192) with
+  // 16: half the shuffles per element (16384 x 4096 bf16: 92 against 103 us, 65536 x 1024: 86 against 104).
   if (v == W) {
-    constexpr int E = sizeof(T) == 2 ? 16 : 8;
-    if ((long long)a.d * (8 + LN_RING * 2 * (long long)sizeof(T)) <= 200 * 1024 && a.d <= 1024 * E)
-      return ln_launch_bwd<T, W, E, true>(a, blocks, st);
+    if ((long long)a.d * (8 + LN_RING * 2 * (long long)sizeof(T)) <= 200 * 1024 && a.d <= 16 * LN_T16)
+      return a.d <= 8192 && (sizeof(T) == 4 || a.d < 1024) ? ln_launch_bwd<T, W, 8, true>(a, blocks, st)
+                                                            : ln_launch_bwd<T, W, 16, true>(a, blocks, st);
     return a.d <= 8192 ? ln_launch_bwd<T, W, 8, false>(a, blocks, st) : ln_launch_bwd<T, W, 16, false>(a, blocks, st);
   }
   if (v == 2) return a.d <= 8192 ? ln_launch_bwd<T, 2, 8, false>(a, blocks, st) : ln_launch_bwd<T, 2, 16, false>(a, blocks, st);

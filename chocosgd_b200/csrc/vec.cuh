@@ -53,4 +53,69 @@ __device__ __forceinline__ void store_any(void* p, int dt, long long i, float v)
   else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// ---- pairs of fp32 numbers: one instruction works on both ------------------------------------------------------------
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float2 f2_get(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float f2_sum(F2 a) {
+  const float2 p = f2_get(a);
+  return p.x + p.y;
+}
+// elements 2 i and 2 i + 1 of a vector
+__device__ __forceinline__ F2 pair_of(const Vec<float, 4>& v, int i) { return f2(v.e[2 * i], v.e[2 * i + 1]); }
+__device__ __forceinline__ F2 pair_of(const Vec<__nv_bfloat16, 8>& v, int i) {
+  const uint32_t w = i == 0 ? v.raw.x : (i == 1 ? v.raw.y : (i == 2 ? v.raw.z : v.raw.w));
+  return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ F2 pair_of(const Vec<__half, 8>& v, int i) {
+  const uint32_t w = i == 0 ? v.raw.x : (i == 1 ? v.raw.y : (i == 2 ? v.raw.z : v.raw.w));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2(f.x, f.y);
+}
+// a vector of pairs, each rounded once (no address of a register is taken: it would end in local memory)
+__device__ __forceinline__ uint32_t pack_bf16x2(F2 a) {
+  const float2 f = f2_get(a);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(F2 a) {
+  const float2 f = f2_get(a);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store_pairs(float* p, const F2 (&a)[2]) {
+  const float2 x = f2_get(a[0]), y = f2_get(a[1]);
+  *reinterpret_cast<float4*>(p) = make_float4(x.x, x.y, y.x, y.y);
+}
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* p, const F2 (&a)[4]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(a[0]), pack_bf16x2(a[1]), pack_bf16x2(a[2]), pack_bf16x2(a[3]));
+}
+__device__ __forceinline__ void store_pairs(__half* p, const F2 (&a)[4]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_f16x2(a[0]), pack_f16x2(a[1]), pack_f16x2(a[2]), pack_f16x2(a[3]));
+}
+
 static inline int dt_bytes(int dt) { return dt == DT_F32 ? 4 : 2; }

@@ -83,10 +83,13 @@ class _LayerNormFn(torch.autograd.Function):
 
 
 def layer_norm_supported(x, weight=None, bias=None) -> bool:
-    return (x.is_cuda and x.dtype in DT and x.dim() >= 1 and 0 < x.shape[-1] < 1 << 24
-            and all(p is None or (p.is_cuda and p.device == x.device and p.dim() == 1 and p.shape[0] == x.shape[-1]
-                                  and p.dtype in (x.dtype, torch.float32)) for p in (weight, bias))
-            and (weight is None or bias is None or weight.dtype == bias.dtype))
+    if not (x.is_cuda and x.dtype in DT and x.dim() >= 1 and 0 < x.shape[-1] < 1 << 24):
+        return False
+    for p in (weight, bias):
+        if p is not None and not (p.dim() == 1 and p.shape[0] == x.shape[-1] and p.device == x.device
+                                  and (p.dtype is x.dtype or p.dtype is torch.float32)):
+            return False
+    return weight is None or bias is None or weight.dtype is bias.dtype
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
@@ -96,6 +99,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
                          "dimension's length on its device, both of its type or both fp32: got "
                          f"{tuple(x.shape)} {x.dtype} {x.device}, "
                          + ", ".join("None" if p is None else f"{tuple(p.shape)} {p.dtype} {p.device}" for p in (weight, bias)))
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     return _lib.on_device(x.device, _LayerNormFn.apply, x, weight, bias, eps)
