@@ -4,7 +4,8 @@
 //   dH = dY W_out          dG = dH U act'(G),  dU = dH act(G)    dX = dG W_in[:F] + dU W_in[F:]
 //   dW_in = [dG | dU]^T X                                        dW_out = dY^T H
 //
-// Six products of one kernel (ffn_gemm_kernel), which differ in the operands' orientation and in the epilogue:
+// Six products of one kernel (ffn_gemm_kernel), in four launches (the last three are independent of each other and share one, so
+// that the tiles of all three fill the machine together), which differ in the operands' orientation and in the epilogue:
 //   gate    both projections of a tile in ONE accumulator (the B tile holds BN / 2 gate rows and the BN / 2 up rows
 //           that belong to them); the epilogue applies activation and product, so G and U meet in registers
 //   dgate   dH stays in the accumulator: the epilogue reads G and U and writes dG and dU
@@ -38,8 +39,7 @@
 
 #define FF_GATE 0
 #define FF_DGATE 1
-#define FF_PLAIN 2
-#define FF_PARTIAL 3         // plain, over a part of k, into fp32 slices that ffn_join_kernel adds up
+#define FF_PLAIN 2           // also over a part of k, into fp32 slices that ffn_join_kernel adds up (k_splits > 1)
 
 __device__ int g_ffn_error;
 
@@ -47,7 +47,7 @@ struct FfnGemm {
   CUtensorMap a, b;
   int M, N;              // output rows (of one part) and columns; gate: N = F
   int k_blocks;          // k-blocks (FF_BK) of one segment
-  int k_splits;          // partial: slices of the k-blocks, one tile each
+  int k_splits;          // plain: slices of the k-blocks, one tile each (1: the result itself)
   int segments;          // dX: 2 (gate and up rows of W_in); else 1
   int m_parts;           // dW_in: 2 (dG and dU); else 1
   int a_parts, b_parts;  // planes per split of the operand (2: gate / up)
@@ -58,8 +58,14 @@ struct FfnGemm {
   int vec16;             // out's rows start on 16-byte boundaries
   long long ldo;
   float* z;              // lane-blocked fp32 (lane_off), ldz columns.  gate: [2] G, U written (null in evaluation);
-  long long ldz;         // dgate: read;  partial: [k_splits][m_parts] written
+  long long ldz;         // dgate: read;  plain in slices: [k_splits][m_parts] written
   long long z_plane;     // floats of one matrix of z
+};
+
+// products of one launch: tiles first[i] .. first[i + 1] - 1 are those of g[i] (gate, dgate: one product)
+struct FfnBatch {
+  FfnGemm g[3];
+  int n, first[4];
 };
 
 // fp32 matrices that only these kernels read (G, U, partial sums) are stored in the order in which a warp of the epilogue
@@ -293,7 +299,7 @@ template <int S, int KIND, int HC, int ACT> struct FfnEpilogue {
       const long long plane = g.M * g.ldo;
       operand<(HC < 32 ? HC : 32)>(c, 0, dg, 0, 2 * plane);
       operand<(HC < 32 ? HC : 32)>(c, 4, du, plane, 2 * plane);
-    } else if (KIND == FF_PARTIAL) {
+    } else if (g.k_splits > 1) {
       if (row0 < g.M && col < g.N) {
         st32b(z + c * 32, reinterpret_cast<const uint32_t*>(v));
         st32b(z + c * 32 + 256, reinterpret_cast<const uint32_t*>(v + 8));
@@ -378,8 +384,7 @@ template <int BN, int S, int KIND, int CG> struct FfnSmem {
 // Tile order: groups of FF_GROUP row tiles, rows fastest within a group, so that the tiles worked on at one time form a
 // block that is about as high as wide and share both operands' panels in L2.
 #define FF_GROUP 8
-__device__ __forceinline__ void ff_tile(int tile, int out_tiles, int tiles_m, int tiles_n, int& tm, int& tn) {
-  tile %= out_tiles;
+__device__ __forceinline__ void ff_tile(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int per_group = FF_GROUP * tiles_n, group = tile / per_group, r = tile - group * per_group;
   const int rows = min(FF_GROUP, tiles_m - group * FF_GROUP);
   tn = r / rows;
@@ -390,26 +395,39 @@ __device__ __forceinline__ void ff_tile(int tile, int out_tiles, int tiles_m, in
 template <int V> struct FfnConst { static constexpr int value = V; };
 template <int KIND, typename F>
 __device__ __forceinline__ void ff_for_act(int act, F f) {
-  if (KIND == FF_PLAIN || KIND == FF_PARTIAL || act == ACT_SILU) f(FfnConst<ACT_SILU>());
+  if (KIND == FF_PLAIN || act == ACT_SILU) f(FfnConst<ACT_SILU>());
   else if (act == ACT_GELU) f(FfnConst<ACT_GELU>());
   else if (act == ACT_RELU) f(FfnConst<ACT_RELU>());
   else f(FfnConst<ACT_SIGMOID>());
 }
 
-// k-blocks [kb0, kb1) of a tile
-template <int KIND>
-__device__ __forceinline__ void ff_slice(const FfnGemm& g, int tile, int out_tiles, int n_kb, int& kb0, int& kb1) {
-  kb0 = 0;
-  kb1 = n_kb;
-  if (KIND == FF_PARTIAL) {
-    const int q = tile / out_tiles;
-    kb0 = (int)((long long)n_kb * q / g.k_splits);
-    kb1 = (int)((long long)n_kb * (q + 1) / g.k_splits);
+// where a tile lies: its product, its first output row and column, its part and slice, its k-blocks [kb0, kb1)
+template <int BN_OUT, int TM, int KIND> struct FfnWhere {
+  const FfnGemm& g;
+  int m0, n0, m_part, slice, kb0, kb1;
+  static __device__ __forceinline__ int which(const FfnBatch& b, int tile) {
+    int i = 0;
+    if (KIND == FF_PLAIN)
+      while (i + 1 < b.n && tile >= b.first[i + 1]) ++i;
+    return i;
   }
-}
+  __device__ __forceinline__ FfnWhere(const FfnBatch& b, int tile, int i) : g(b.g[i]) {
+    const int tiles_m = (g.M + TM - 1) / TM, tiles_n = (g.N + BN_OUT - 1) / BN_OUT, out_tiles = tiles_m * g.m_parts * tiles_n;
+    int local = tile - b.first[i], tm, tn;
+    slice = KIND == FF_PLAIN ? local / out_tiles : 0;
+    local -= slice * out_tiles;
+    ff_tile(local, tiles_m * g.m_parts, tiles_n, tm, tn);
+    m_part = tm / tiles_m;
+    m0 = (tm - m_part * tiles_m) * TM;
+    n0 = tn * BN_OUT;
+    const int n_kb = g.k_blocks * g.segments;
+    kb0 = KIND == FF_PLAIN ? (int)((long long)n_kb * slice / g.k_splits) : 0;
+    kb1 = KIND == FF_PLAIN ? (int)((long long)n_kb * (slice + 1) / g.k_splits) : n_kb;
+  }
+};
 
 template <int BN, int S, int KIND, int CG>
-__global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1) ffn_gemm_kernel(const __grid_constant__ FfnGemm g) {
+__global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1) ffn_gemm_kernel(const __grid_constant__ FfnBatch batch) {
   typedef FfnSmem<BN, S, KIND, CG> L;
   extern __shared__ uint8_t smem_raw[];
   // 1024-byte alignment: the swizzle pattern is a function of the shared-memory address bits
@@ -427,10 +445,8 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
-  const int tiles_m = (g.M + TM - 1) / TM, tiles_n = (g.N + BN_OUT - 1) / BN_OUT;
-  const int out_tiles = tiles_m * g.m_parts * tiles_n;
-  const int n_tiles = KIND == FF_PARTIAL ? out_tiles * g.k_splits : out_tiles;
-  const int n_kb_all = g.k_blocks * g.segments;
+  typedef FfnWhere<BN_OUT, TM, KIND> Where;
+  const int n_tiles = batch.first[batch.n];
   const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
 
   if (threadIdx.x == 0) {
@@ -462,12 +478,11 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
     uint32_t it = 0, s = 0, phase = 1;      // stage and the parity of its `empty` barrier (the first round passes at once)
     bool ok = true;
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step) {
-      int tm, tn, kb0, kb1;
-      ff_slice<KIND>(g, tile, out_tiles, n_kb_all, kb0, kb1);
-      ff_tile(tile, out_tiles, tiles_m * g.m_parts, tiles_n, tm, tn);
-      const int n0 = tn * BN_OUT, m_part = tm / tiles_m, m0 = (tm % tiles_m) * TM + (int)rank * FF_BM;
+      const Where at(batch, tile, Where::which(batch, tile));
+      const FfnGemm& g = at.g;
+      const int n0 = at.n0, m_part = at.m_part, m0 = at.m0 + (int)rank * FF_BM;
       {
-        for (int i = kb0; i < kb1; ++i) {
+        for (int i = at.kb0; i < at.kb1; ++i) {
           const int seg = i >= g.k_blocks ? 1 : 0, k0 = (i - seg * g.k_blocks) * BK;
           const int part_a = g.m_parts > 1 ? m_part : (g.a_parts > 1 ? seg : 0), part_b = g.b_parts > 1 ? seg : 0;
           ok = __all_sync(0xffffffffu, mbar_wait(empty + s, phase) && *abort_flag == 0);
@@ -520,23 +535,23 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
     }
   } else if (warp == L::EPI + 1 && rank == 0) {
     // ---------------- MMA issuer (of a pair: the leader's) ----------------
-    // instruction descriptor: fp32 accumulate, operand type, majorness bits, N >> 3, M >> 4
-    const uint32_t type = g.fp16 ? 0u : 1u;
-    const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)g.a_mn << 15) | ((uint32_t)g.b_mn << 16) |
-                           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
-    // K-major: 16 k = 32 bytes further inside the (64- or 128-byte) row, groups of 8 rows apart; MN-major: 16 k = 16 rows of
-    // 128 bytes, 8-k groups 1024 bytes apart, blocks of 64 MN elements BK rows apart.  Descriptors count in 16 bytes.
-    const uint32_t a_step = (g.a_mn ? 2048 : 32) >> 4, b_step = (g.b_mn ? 2048 : 32) >> 4;
-    const uint32_t base = smem_u32(smem);
-    const uint64_t da0 = g.a_mn ? make_desc(base, BK * 128, 1024) : make_desc(base, 16, BK * 16, BK == 32 ? 4 : 2);
-    const uint64_t db0 = g.b_mn ? make_desc(base + S * L::A_TILE, BK * 128, 1024)
-                                : make_desc(base + S * L::A_TILE, 16, BK * 16, BK == 32 ? 4 : 2);
     uint32_t s = 0, phase = 0, chunk = 0;
+    const uint32_t base = smem_u32(smem);
     bool ok = true;
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step) {
-      int kb0, kb1;
-      ff_slice<KIND>(g, tile, out_tiles, n_kb_all, kb0, kb1);
-      const int n_kb = kb1 - kb0;
+      const Where at(batch, tile, Where::which(batch, tile));
+      const FfnGemm& g = at.g;
+      const int n_kb = at.kb1 - at.kb0;
+      // instruction descriptor: fp32 accumulate, operand type, majorness bits, N >> 3, M >> 4
+      const uint32_t type = g.fp16 ? 0u : 1u;
+      const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)g.a_mn << 15) | ((uint32_t)g.b_mn << 16) |
+                             ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+      // K-major: 16 k = 32 bytes further inside the (64- or 128-byte) row, groups of 8 rows apart; MN-major: 16 k = 16 rows of
+      // 128 bytes, 8-k groups 1024 bytes apart, blocks of 64 MN elements BK rows apart.  Descriptors count in 16 bytes.
+      const uint32_t a_step = (g.a_mn ? 2048 : 32) >> 4, b_step = (g.b_mn ? 2048 : 32) >> 4;
+      const uint64_t da0 = g.a_mn ? make_desc(base, BK * 128, 1024) : make_desc(base, 16, BK * 16, BK == 32 ? 4 : 2);
+      const uint64_t db0 = g.b_mn ? make_desc(base + S * L::A_TILE, BK * 128, 1024)
+                                  : make_desc(base + S * L::A_TILE, 16, BK * 16, BK == 32 ? 4 : 2);
       for (int i = 0; i < n_kb; ++i) {
         const uint32_t buf = chunk & 1;
         const bool first = S == 3 || i == 0, last = S == 3 || i == n_kb - 1;      // S = 3: every k-block has its accumulator
@@ -577,14 +592,13 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
     uint32_t chunk = 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     for (int tile = first_tile; tile < n_tiles; tile += tile_step) {
-      int tm, tn, kb0, kb1;
-      ff_slice<KIND>(g, tile, out_tiles, n_kb_all, kb0, kb1);
-      ff_tile(tile, out_tiles, tiles_m * g.m_parts, tiles_n, tm, tn);
-      const int m_part = tm / tiles_m;
-      const int z_index = KIND == FF_PARTIAL ? tile / out_tiles * g.m_parts + m_part : m_part;
-      const int row0 = (tm % tiles_m) * TM + (int)rank * FF_BM + (warp & 3) * 32, col0 = tn * BN_OUT + half * HC;
-      float* z = KIND == FF_PLAIN || g.z == nullptr
-                     ? nullptr : g.z + (KIND == FF_PARTIAL ? z_index * g.z_plane : 0) + lane_off(row0 + lane, col0, g.ldz);
+      const Where at(batch, tile, Where::which(batch, tile));
+      const FfnGemm& g = at.g;
+      const int m_part = at.m_part;
+      const int row0 = at.m0 + (int)rank * FF_BM + (warp & 3) * 32, col0 = at.n0 + half * HC;
+      float* z = nullptr;
+      if (g.z != nullptr)
+        z = g.z + (KIND == FF_PLAIN ? (at.slice * g.m_parts + m_part) * g.z_plane : 0) + lane_off(row0 + lane, col0, g.ldz);
       const int z_cols = row0 < g.M ? g.N - col0 : 0;      // columns of z that exist
       bool stop = false;
       if (S == 3) {
@@ -593,7 +607,7 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
         float acc[NA];
 #pragma unroll
         for (int c = 0; c < NA; ++c) acc[c] = 0.f;
-        for (int i = kb0; i < kb1; ++i, ++chunk) {
+        for (int i = at.kb0; i < at.kb1; ++i, ++chunk) {
           const uint32_t buf = chunk & 1;
           const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
           if (ff_epi_bar_or<L::EPI>(bad)) { stop = true; break; }
@@ -806,23 +820,32 @@ static int ffn_map(CUtensorMap* map, const FfnOperand& o, int fp16, int mn_major
   return r == CUDA_SUCCESS ? 0 : -12;
 }
 
+struct FfnOperands {
+  FfnOperand a, b;
+};
+
 template <int BN, int S, int KIND, int CG>
-static int ffn_launch_t(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
-  void (*kernel)(FfnGemm) = ffn_gemm_kernel<BN, S, KIND, CG>;
+static int ffn_launch_t(FfnBatch& batch, const FfnOperands* o, cudaStream_t st) {
+  void (*kernel)(FfnBatch) = ffn_gemm_kernel<BN, S, KIND, CG>;
   typedef FfnSmem<BN, S, KIND, CG> L;
   constexpr int smem = L::BYTES;
   // before the tensor maps: a runtime call makes the device's context current in a thread that has not used it yet
   // (autograd's), without which the driver refuses to encode a map
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
-  int rc = ffn_map(&g.a, a, g.fp16, g.a_mn, FF_BM, FF_BK(S));
-  if (rc) return rc;
-  rc = ffn_map(&g.b, b, g.fp16, g.b_mn, KIND == FF_GATE ? BN / 2 : BN / CG, FF_BK(S));
-  if (rc) return rc;
   const int bn_out = KIND == FF_GATE ? BN / 2 : BN;
-  const long long tiles = (long long)((g.M + CG * FF_BM - 1) / (CG * FF_BM)) * g.m_parts * ((g.N + bn_out - 1) / bn_out) *
-                          (KIND == FF_PARTIAL ? g.k_splits : 1);
-  if (tiles > 0x3fffffffLL) return -1;
+  long long tiles = 0;
+  for (int i = 0; i < batch.n; ++i) {
+    FfnGemm& g = batch.g[i];
+    int rc = ffn_map(&g.a, o[i].a, g.fp16, g.a_mn, FF_BM, FF_BK(S));
+    if (rc) return rc;
+    rc = ffn_map(&g.b, o[i].b, g.fp16, g.b_mn, KIND == FF_GATE ? BN / 2 : BN / CG, FF_BK(S));
+    if (rc) return rc;
+    batch.first[i] = (int)tiles;
+    tiles += (long long)((g.M + CG * FF_BM - 1) / (CG * FF_BM)) * g.m_parts * ((g.N + bn_out - 1) / bn_out) * g.k_splits;
+    if (tiles > 0x3fffffffLL) return -1;
+  }
+  batch.first[batch.n] = (int)tiles;
   const int most = sm_count() / CG, grid = CG * (tiles < most ? (int)tiles : most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -844,95 +867,143 @@ static int ffn_launch_t(FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cu
   }
   cfg.attrs = at;
   cfg.numAttrs = n;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, g);
+  return (int)cudaLaunchKernelEx(&cfg, kernel, batch);
 }
 
-// Which tile a product runs with, by its time in SM cycles:  rounds x (64-k blocks x step + exposed epilogue), where
-//   rounds    tiles per SM (pair), rounded up
+// Which tile a launch runs with, by its time in SM cycles:  tiles per SM (pair) x (64-k blocks x step + exposed epilogue), where
 //   step      the slower of multiplying (1024 multiply-adds x 4 per cycle and SM; six times for three planes) and of fetching
 //             the operands (measured: about 58 bytes per cycle and SM from L2 when all SMs fetch)
-//   epilogue  runs under the next tile's multiplications for 16-bit operands, not for three planes (whose sums are in the
-//             epilogue's registers)
-// and, for a plain product cut into slices of k, the partial sums' second pass (a launch, then 4 bytes of each written and read).
-struct FfnTile {
-  int bn, cg, splits;
+//   epilogue  (measured) runs under the next tile's multiplications for 16-bit operands, not for three planes (whose sums are in
+//             the epilogue's registers)
+// One product: whole rounds.  Several: their tiles follow one another, so the average load and half of the largest tile.
+// A plain product can be cut into slices of k (not 256 wide: there the tiles are many), which costs the partial sums' second
+// pass: a launch, then 4 bytes of each written and read.
+struct FfnProduct {
+  int M, m_parts, cols;
+  long long k64;
 };
-static double ffn_cost(const FfnTile& t, int S, int kind, int M, int m_parts, int cols, long long k64) {
-  const int sms = sm_count() / t.cg, tm = FF_BM * t.cg;
-  const double tiles = (double)((M + tm - 1) / tm) * m_parts * ((cols + t.bn - 1) / t.bn) * t.splits;
-  const double rounds = (double)(long long)((tiles + sms - 1) / sms);
-  const double mul = 2.0 * t.bn * (S == 3 ? 6 : 1), fetch = S * (FF_BM + t.bn / t.cg) * 128.0 / 58.0;
-  const double step = mul > fetch ? mul : fetch, main = (double)((k64 + t.splits - 1) / t.splits) * step;
-  const double epi = t.bn * (kind == FF_DGATE ? (S == 3 ? 180.0 : 70.0) : 45.0);
-  double c = S == 3 ? rounds * (main + epi) : rounds * (main > epi ? main : epi) + epi;
-  c += 3000.0;                                               // launch, first loads
-  if (t.splits > 1) c += 5000.0 + 8.0 * t.splits * m_parts * M * cols / (30.0 * sm_count());
-  return c;
+struct FfnPlan {
+  int bn, cg, splits[3];
+};
+static double ffn_tile_cost(int bn, int cg, int S, int kind, long long k64) {
+  const double mul = 2.0 * bn * (S == 3 ? 6 : 1), fetch = S * (FF_BM + bn / cg) * 128.0 / 58.0;
+  const double main = (double)k64 * (mul > fetch ? mul : fetch);
+  double epi = bn * (kind == FF_DGATE ? 70.0 : 45.0);
+  if (S == 3) epi = kind == FF_DGATE ? 12000.0 + 110.0 * bn : (kind == FF_GATE ? 6000.0 + 30.0 * bn : 2000.0 + 90.0 * bn);
+  return S == 3 ? main + epi : (main > epi ? main : epi);
 }
-// the cheapest of: pairs 256 / 128 wide, single CTAs 128 / 64 wide; a plain product also in up to 16 slices of at least 256 k
-// (not 256 wide: there the tiles are many)
-static FfnTile ffn_tile_for(int S, int kind, int M, int m_parts, int cols, long long k64) {
-  static const FfnTile shapes[4] = {{256, 2, 1}, {128, 2, 1}, {128, 1, 1}, {64, 1, 1}};
-  FfnTile best = shapes[0];
-  double cost = 1e300;
+static FfnPlan ffn_plan(int S, int kind, const FfnProduct* p, int n) {
+  static const int shapes[4][2] = {{256, 2}, {128, 2}, {128, 1}, {64, 1}};
+  FfnPlan best = {256, 2, {1, 1, 1}};
+  double best_cost = 1e300;
   for (int i = 0; i < 4; ++i) {
-    if (shapes[i].cg == 2 && M <= FF_BM) continue;
-    // 1, 2, 3, 4, 6, 8, 12, 16 slices
-    for (int q = 1; q <= (kind == FF_PLAIN && (i == 1 || i == 3) ? 16 : 1); q += q < 4 ? 1 : (q < 8 ? 2 : 4)) {
-      if (q > 1 && (k64 / q < 4 || (long long)m_parts * ((M + 31) / 32) > 65535)) break;    // 65535: grid of ffn_join_kernel
-      FfnTile t = shapes[i];
-      t.splits = q;
-      const double c = ffn_cost(t, S, kind, M, m_parts, cols, k64);
-      if (c < cost) { cost = c; best = t; }
+    const int bn = shapes[i][0], cg = shapes[i][1], tm = FF_BM * cg, units = sm_count() / cg;
+    bool low = true;
+    double tiles[3], total = 0;
+    for (int j = 0; j < n; ++j) {
+      low = low && p[j].M <= FF_BM;
+      tiles[j] = (double)((p[j].M + tm - 1) / tm) * p[j].m_parts * ((p[j].cols + bn - 1) / bn);
+      total += tiles[j] * ffn_tile_cost(bn, cg, S, kind, p[j].k64);
+    }
+    if (low && cg == 2) continue;
+    for (int most = 1; most <= (kind == FF_PLAIN && bn < 256 ? 16 : 1); most += most < 4 ? 1 : (most < 8 ? 2 : 4)) {
+      // slices: one product `most`; several: those whose tiles are longer than 1 / most of an SM's load are cut to that
+      FfnPlan plan = {bn, cg, {1, 1, 1}};
+      double load = 0, largest = 0, join = 0;
+      bool cut = false;
+      for (int j = 0; j < n; ++j) {
+        long long q = most;
+        if (n > 1) q = (long long)(ffn_tile_cost(bn, cg, S, kind, p[j].k64) * units * most / total);
+        if (q > p[j].k64 / 4) q = p[j].k64 / 4;
+        if (q > 16) q = 16;
+        if (most == 1 || q < 1 || (long long)p[j].m_parts * ((p[j].M + 31) / 32) > 65535) q = 1;      // 65535: grid of ffn_join_kernel
+        plan.splits[j] = (int)q;
+        const double c = ffn_tile_cost(bn, cg, S, kind, (p[j].k64 + q - 1) / q);
+        load += tiles[j] * q * c;
+        if (c > largest) largest = c;
+        if (q > 1) {
+          cut = true;
+          join += 5000.0 + 8.0 * q * p[j].m_parts * p[j].M * p[j].cols / (30.0 * sm_count());
+        }
+      }
+      if (most > 1 && !cut) continue;
+      double cost = join + 3000.0;                       // launch, first loads
+      if (n == 1) cost += largest * (double)(long long)((tiles[0] * plan.splits[0] + units - 1) / units);
+      else cost += load / units + 0.5 * largest;
+      if (cost < best_cost) { best_cost = cost; best = plan; }
     }
   }
   return best;
 }
 template <int S, int KIND>
-static int ffn_launch(const FfnTile& t, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
-  if (t.cg == 2) return t.bn == 256 ? ffn_launch_t<256, S, KIND, 2>(g, a, b, st) : ffn_launch_t<128, S, KIND, 2>(g, a, b, st);
-  return t.bn == 128 ? ffn_launch_t<128, S, KIND, 1>(g, a, b, st) : ffn_launch_t<64, S, KIND, 1>(g, a, b, st);
+static int ffn_launch(const FfnPlan& t, FfnBatch& batch, const FfnOperands* o, cudaStream_t st) {
+  if (t.cg == 2) return t.bn == 256 ? ffn_launch_t<256, S, KIND, 2>(batch, o, st) : ffn_launch_t<128, S, KIND, 2>(batch, o, st);
+  return t.bn == 128 ? ffn_launch_t<128, S, KIND, 1>(batch, o, st) : ffn_launch_t<64, S, KIND, 1>(batch, o, st);
 }
 
 static long long ffn_plane(int M, int N) { return (long long)((M + 31) / 32 * 32) * ((N + 15) / 16 * 16); }
-static long long ffn_k64(int S, int k_blocks, int segments) { return ((long long)k_blocks * segments * FF_BK(S) + 63) / 64; }
 static int ffn_k_blocks(int S, int k) { return (k + FF_BK(S) - 1) / FF_BK(S); }
-// floats of partial sums that a plain product needs
-static long long ffn_partial_floats(int S, int M, int m_parts, int N, int k, int segments) {
-  const FfnTile t = ffn_tile_for(S, FF_PLAIN, M, m_parts, N, ffn_k64(S, ffn_k_blocks(S, k), segments));
-  return t.splits > 1 ? t.splits * m_parts * ffn_plane(M, N) : 0;
+static FfnProduct ffn_product(int S, int M, int m_parts, int cols, int k, int segments) {
+  return {M, m_parts, cols, ((long long)ffn_k_blocks(S, k) * segments * FF_BK(S) + 63) / 64};
+}
+// floats of partial sums that plain products need
+static long long ffn_partial_floats(const FfnPlan& plan, const FfnProduct* p, int n) {
+  long long floats = 0;
+  for (int j = 0; j < n; ++j)
+    if (plan.splits[j] > 1) floats += plan.splits[j] * p[j].m_parts * ffn_plane(p[j].M, p[j].cols);
+  return floats;
+}
+// the products of the two plain launches: Y;  dX, dW_in, dW_out
+static FfnProduct ffn_y_product(int S, int m, int f, int n) { return ffn_product(S, m, 1, n, f, 1); }
+static void ffn_grad_products(int S, int m, int d, int f, int n, FfnProduct (&p)[3]) {
+  p[0] = ffn_product(S, m, 1, d, f, 2);
+  p[1] = ffn_product(S, f, 2, d, m, 1);
+  p[2] = ffn_product(S, n, 1, f, m, 1);
 }
 
+// gate, dgate
 template <int KIND>
-static int ffn_gemm(int S, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, cudaStream_t st) {
-  const FfnTile t = ffn_tile_for(S, KIND, g.M, g.m_parts, KIND == FF_GATE ? 2 * g.N : g.N, ffn_k64(S, g.k_blocks, g.segments));
-  return S == 3 ? ffn_launch<3, KIND>(t, g, a, b, st) : ffn_launch<1, KIND>(t, g, a, b, st);
+static int ffn_gemm(int S, const FfnGemm& g, const FfnOperand& a, const FfnOperand& b, int k, cudaStream_t st) {
+  const FfnProduct p = ffn_product(S, g.M, 1, KIND == FF_GATE ? 2 * g.N : g.N, k, 1);
+  const FfnPlan plan = ffn_plan(S, KIND, &p, 1);
+  FfnBatch batch = {};
+  batch.g[0] = g;
+  batch.g[0].k_splits = 1;
+  batch.n = 1;
+  const FfnOperands o = {a, b};
+  return S == 3 ? ffn_launch<3, KIND>(plan, batch, &o, st) : ffn_launch<1, KIND>(plan, batch, &o, st);
 }
-// plain product of S operand planes into out [m_parts M, N]; partial: scratch of ffn_partial_floats
-static int ffn_plain(int S, FfnGemm& g, const FfnOperand& a, const FfnOperand& b, void* out, int dt, float* partial, cudaStream_t st) {
-  g.out = out;
-  g.ldo = g.N;
-  g.vec16 = (((uintptr_t)out | (uintptr_t)((long long)g.N * dt_bytes(dt))) & 15) == 0;
-  const FfnTile t = ffn_tile_for(S, FF_PLAIN, g.M, g.m_parts, g.N, ffn_k64(S, g.k_blocks, g.segments));
-  g.k_splits = t.splits;
-  if (t.splits == 1) return S == 3 ? ffn_launch<3, FF_PLAIN>(t, g, a, b, st) : ffn_launch<1, FF_PLAIN>(t, g, a, b, st);
-  if (partial == nullptr) return -1;
-  g.z = partial;
-  g.ldz = (g.N + 15) / 16 * 16;
-  g.z_plane = ffn_plane(g.M, g.N);
-  int rc;
-  if (t.cg == 2) rc = S == 3 ? ffn_launch_t<128, 3, FF_PARTIAL, 2>(g, a, b, st) : ffn_launch_t<128, 1, FF_PARTIAL, 2>(g, a, b, st);
-  else rc = S == 3 ? ffn_launch_t<64, 3, FF_PARTIAL, 1>(g, a, b, st) : ffn_launch_t<64, 1, FF_PARTIAL, 1>(g, a, b, st);
-  if (rc) return rc;
-  const dim3 grid((g.N + 63) / 64, g.m_parts * ((g.M + 31) / 32)), block(256);
-  if (dt == DT_F32)
-    return (int)launch_k(ffn_join_kernel<float>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, g.k_splits, g.m_parts,
-                         g.M, g.N, (float*)out);
-  if (dt == DT_BF16)
-    return (int)launch_k(ffn_join_kernel<__nv_bfloat16>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, g.k_splits,
-                         g.m_parts, g.M, g.N, (__nv_bfloat16*)out);
-  return (int)launch_k(ffn_join_kernel<__half>, grid, block, 0, st, (const float*)partial, g.ldz, g.z_plane, g.k_splits, g.m_parts,
-                       g.M, g.N, (__half*)out);
+// plain products of S operand planes, g[i].out [m_parts M, N]; partial: scratch of ffn_partial_floats
+static int ffn_plain(int S, const FfnPlan& plan, FfnBatch& batch, const int* index, const FfnOperands* o, int dt, float* partial,
+                     cudaStream_t st) {
+  for (int i = 0; i < batch.n; ++i) {
+    FfnGemm& g = batch.g[i];
+    g.ldo = g.N;
+    g.vec16 = (((uintptr_t)g.out | (uintptr_t)((long long)g.N * dt_bytes(dt))) & 15) == 0;
+    g.k_splits = plan.splits[index[i]];
+    if (g.k_splits == 1) continue;
+    if (partial == nullptr) return -1;
+    g.z = partial;
+    g.ldz = (g.N + 15) / 16 * 16;
+    g.z_plane = ffn_plane(g.M, g.N);
+    partial += g.k_splits * g.m_parts * g.z_plane;
+  }
+  int rc = S == 3 ? ffn_launch<3, FF_PLAIN>(plan, batch, o, st) : ffn_launch<1, FF_PLAIN>(plan, batch, o, st);
+  for (int i = 0; i < batch.n && !rc; ++i) {
+    const FfnGemm& g = batch.g[i];
+    if (g.k_splits == 1) continue;
+    const dim3 grid((g.N + 63) / 64, g.m_parts * ((g.M + 31) / 32)), block(256);
+    if (dt == DT_F32)
+      rc = (int)launch_k(ffn_join_kernel<float>, grid, block, 0, st, (const float*)g.z, g.ldz, g.z_plane, g.k_splits, g.m_parts,
+                         g.M, g.N, (float*)g.out);
+    else if (dt == DT_BF16)
+      rc = (int)launch_k(ffn_join_kernel<__nv_bfloat16>, grid, block, 0, st, (const float*)g.z, g.ldz, g.z_plane, g.k_splits,
+                         g.m_parts, g.M, g.N, (__nv_bfloat16*)g.out);
+    else
+      rc = (int)launch_k(ffn_join_kernel<__half>, grid, block, 0, st, (const float*)g.z, g.ldz, g.z_plane, g.k_splits, g.m_parts,
+                         g.M, g.N, (__half*)g.out);
+  }
+  return rc;
 }
 
 // A matrix the products can read: itself, or its image `dst` in the workspace, which `images` then has to make (src null:
@@ -977,11 +1048,10 @@ static bool ffn_shape_ok(const FfnShape& s) {
 extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt, int backward) {
   const int S = dt == DT_F32 ? 3 : 1;
   if (m <= 0 || d <= 0 || f <= 0 || n <= 0) return 0;
-  if (!backward) return ffn_partial_floats(S, m, 1, n, f, 1);
-  long long a = ffn_partial_floats(S, m, 1, d, f, 2);
-  const long long b = ffn_partial_floats(S, f, 2, d, m, 1), c = ffn_partial_floats(S, n, 1, f, m, 1);
-  a = a > b ? a : b;
-  return a > c ? a : c;
+  FfnProduct p[3];
+  if (backward) ffn_grad_products(S, m, d, f, n, p);
+  else p[0] = ffn_y_product(S, m, f, n);
+  return ffn_partial_floats(ffn_plan(S, FF_PLAIN, p, backward ? 3 : 1), p, backward ? 3 : 1);
 }
 
 // most tokens of an evaluation pass that the form for few tokens takes (`few` of gated_ffn_forward)
@@ -1031,12 +1101,19 @@ extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
   g.b_parts = 2;
   g.M = m; g.N = f; g.k_blocks = ffn_k_blocks(S, d);
   g.out = h; g.ldo = pad16(f); g.vec16 = 1; g.z = z; g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
-  rc = ffn_gemm<FF_GATE>(S, g, ox, oi, st);
+  rc = ffn_gemm<FF_GATE>(S, g, ox, oi, d, st);
   if (rc) return rc;
-  const FfnOperand oh = {h, m, f, 1, S, pad16(f)};
-  g.b_parts = 1;
-  g.N = n; g.k_blocks = ffn_k_blocks(S, f);
-  return ffn_plain(S, g, oh, oo, y, dt, partial, st);
+  const FfnOperands o = {{h, m, f, 1, S, pad16(f)}, oo};
+  FfnBatch batch = {};
+  batch.n = 1;
+  FfnGemm& b = batch.g[0];
+  b.fp16 = g.fp16;
+  b.segments = b.m_parts = b.a_parts = b.b_parts = 1;
+  b.M = m; b.N = n; b.k_blocks = ffn_k_blocks(S, f);
+  b.out = y;
+  const FfnProduct p = ffn_y_product(S, m, f, n);
+  const int index = 0;
+  return ffn_plain(S, ffn_plan(S, FF_PLAIN, &p, 1), batch, &index, &o, dt, partial, st);
 }
 
 // x, w_in, w_out: as in the forward pass; where an image is given it holds the forward pass' image already.
@@ -1086,28 +1163,41 @@ extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
   base.fp16 = dt == DT_F16;
   base.act = act;
   base.segments = base.m_parts = base.a_parts = base.b_parts = 1;
-  FfnGemm g = base;
   if (dx != nullptr || dw_in != nullptr) {
+    FfnGemm g = base;
     g.M = m; g.N = f; g.k_blocks = ffn_k_blocks(S, n); g.b_mn = 1;
     g.out = dz; g.ldo = pad16(f); g.vec16 = 1; g.z = z; g.ldz = pad16(f); g.z_plane = ffn_plane(m, f);
-    if ((rc = ffn_gemm<FF_DGATE>(S, g, oy, oo, st))) return rc;
+    if ((rc = ffn_gemm<FF_DGATE>(S, g, oy, oo, n, st))) return rc;
   }
+  // the plan is that of all three products whichever are wanted: a gradient's bits do not depend on the others
+  FfnProduct p[3];
+  ffn_grad_products(S, m, d, f, n, p);
+  const FfnPlan plan = ffn_plan(S, FF_PLAIN, p, 3);
+  FfnBatch batch = {};
+  FfnOperands o[3];
+  int index[3];
   if (dx != nullptr) {
-    g = base;
+    FfnGemm& g = batch.g[batch.n] = base;
     g.M = m; g.N = d; g.k_blocks = ffn_k_blocks(S, f); g.segments = 2; g.a_parts = g.b_parts = 2; g.b_mn = 1;
-    if ((rc = ffn_plain(S, g, oz, oi, dx, dt, partial, st))) return rc;
+    g.out = dx;
+    o[batch.n] = {oz, oi};
+    index[batch.n++] = 0;
   }
   if (dw_in != nullptr) {
-    g = base;
+    FfnGemm& g = batch.g[batch.n] = base;
     g.M = f; g.N = d; g.k_blocks = ffn_k_blocks(S, m); g.m_parts = g.a_parts = 2; g.a_mn = g.b_mn = 1;
-    if ((rc = ffn_plain(S, g, oz, ox, dw_in, dt, partial, st))) return rc;
+    g.out = dw_in;
+    o[batch.n] = {oz, ox};
+    index[batch.n++] = 1;
   }
   if (dw_out != nullptr) {
-    g = base;
+    FfnGemm& g = batch.g[batch.n] = base;
     g.M = n; g.N = f; g.k_blocks = ffn_k_blocks(S, m); g.a_mn = g.b_mn = 1;
-    if ((rc = ffn_plain(S, g, oy, oh, dw_out, dt, partial, st))) return rc;
+    g.out = dw_out;
+    o[batch.n] = {oy, oh};
+    index[batch.n++] = 2;
   }
-  return 0;
+  return batch.n ? ffn_plain(S, plan, batch, index, o, dt, partial, st) : 0;
 }
 
 // 0, or 1 after a bounded wait of a kernel on the current device ran out (synchronises)
