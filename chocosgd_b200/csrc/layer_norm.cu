@@ -645,7 +645,9 @@ static int ln_fwd_ring(const LnArgs& a, cudaStream_t st, bool* done) {
 template <typename T, int V>
 static int ln_fwd(const LnArgs& a, cudaStream_t st) {
   if (a.d > 256 * V * 4 || (a.n >= 8LL * sm_count() && a.d > 32 * V * 4)) {
-    if (a.d > 256 * V * 16) return ln_launch_fwd<T, V, 64 / V>(a, st);      // element-wise rows: up to 64 per lane
+    if constexpr (V < 4) {
+      if (a.d > 256 * V * 16) return ln_launch_fwd<T, V, 64 / V>(a, st);      // narrow accesses: up to 64 elements per lane
+    }
     return ln_launch_fwd<T, V, 16>(a, st);
   }
   if (a.d > 256 * V * 2) return ln_launch_fwd<T, V, 4>(a, st);

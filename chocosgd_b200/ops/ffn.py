@@ -3,8 +3,10 @@
 ``gated_ffn(x, w_in, w_out, act="silu")`` computes ``(act(x Wg^T) * (x Wu^T)) Wout^T`` with ``w_in = [Wg; Wu]`` of shape
 ``[2 F, D]`` (gate rows first) and ``w_out`` of shape ``[N, F]``; ``x`` has any leading shape.  All three are bf16, fp16 or fp32 and of
 one type.  16-bit operands are multiplied as they are with fp32 accumulators, the hidden activation is rounded once to their type;
-fp32 operands are split into three bf16 parts each and keep fp32 accuracy.  Rows that do not start on 16-byte boundaries (and
-fp32 operands) are re-laid into an image of the operand first; the backward pass uses the forward pass' images."""
+fp32 operands are split into three bf16 parts each and keep fp32 accuracy (a row that holds an infinity gives
+non-finite results, not always the infinity itself; so does a hidden value above fp16's range with fp16 operands).  Rows that do not start on 16-byte boundaries (and
+fp32 operands) are re-laid into an image of the operand first; the backward pass uses the forward pass' images.  Without a gradient
+and for few tokens (8, fp32: 64) the weights are read once as they are, without tensor cores."""
 from __future__ import annotations
 
 import ctypes
@@ -12,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .norm import DT, ptr, rows_of
+from .norm import DT, pitch, ptr, rows_of
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 
@@ -44,7 +46,7 @@ def _pad32(n: int) -> int:
 
 
 def _aligned(t: torch.Tensor) -> bool:
-    return t.dtype != torch.float32 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0
+    return t.dtype != torch.float32 and t.data_ptr() % 16 == 0 and pitch(t) % 8 == 0
 
 
 class _Layout:
@@ -57,9 +59,6 @@ class _Layout:
         at = self.size
         self.size += (nbytes + 255) // 256 * 256
         return at
-
-    def scratch(self, floats: int):
-        return self.add(4 * floats) if floats else None
 
     def image(self, t: torch.Tensor):
         """Room for the operand image of a matrix, or None where it is read as it is."""
@@ -89,13 +88,14 @@ class _GatedFfnFn(torch.autograd.Function):
             img = [lay.image(t) for t in (x2, wi, wo)]
             h = lay.add((3 if x.dtype == torch.float32 else 1) * m * _pad16(f) * 2)
             z = lay.add(2 * _pad32(m) * _pad16(f) * 4) if train else None
-            partial = lay.scratch(lib.gated_ffn_partial_floats(m, d, f, n, dt, 0))
+            floats = lib.gated_ffn_partial_floats(m, d, f, n, dt, 0)
+            partial = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
         buf = torch.empty(lay.size, dtype=torch.uint8, device=x.device)
         if m:
             b = buf.data_ptr()
             rc = _lib.packed("gated_ffn_forward", "21q")(
-                x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
-                wo.data_ptr(), wo.stride(0), _at(b, img[2]), b + h, _at(b, z), _at(b, partial),
+                x2.data_ptr(), pitch(x2), _at(b, img[0]), wi.data_ptr(), pitch(wi), _at(b, img[1]),
+                wo.data_ptr(), pitch(wo), _at(b, img[2]), b + h, _at(b, z), ptr(partial),
                 y.data_ptr(), m, d, f, n, act, dt, int(few), _lib.raw_stream(x2.device))
             if rc:
                 raise RuntimeError(f"gated_ffn_forward failed with code {rc}")
@@ -122,17 +122,18 @@ class _GatedFfnFn(torch.autograd.Function):
             lay = _Layout()
             dy_img = lay.image(dy2)
             dz = lay.add((3 if x2.dtype == torch.float32 else 1) * 2 * m * _pad16(f) * 2)
-            partial = lay.scratch(lib.gated_ffn_partial_floats(m, d, f, n, DT[x2.dtype], 1))
+            floats = lib.gated_ffn_partial_floats(m, d, f, n, DT[x2.dtype], 1)
+            partial = lay.add(4 * floats) if floats else None
             scratch = torch.empty(lay.size, dtype=torch.uint8, device=x2.device)
             b, s = buf.data_ptr(), scratch.data_ptr()
             rc = _lib.packed("gated_ffn_backward", "26q")(
-                x2.data_ptr(), x2.stride(0), _at(b, img[0]), wi.data_ptr(), wi.stride(0), _at(b, img[1]),
-                wo.data_ptr(), wo.stride(0), _at(b, img[2]), dy2.data_ptr(), dy2.stride(0),
+                x2.data_ptr(), pitch(x2), _at(b, img[0]), wi.data_ptr(), pitch(wi), _at(b, img[1]),
+                wo.data_ptr(), pitch(wo), _at(b, img[2]), dy2.data_ptr(), pitch(dy2),
                 _at(s, dy_img), b + h, b + z, s + dz, _at(s, partial), ptr(dx), ptr(dwi),
                 ptr(dwo), m, d, f, n, ctx.act, DT[x2.dtype], _lib.raw_stream(x2.device))
             if rc:
                 raise RuntimeError(f"gated_ffn_backward failed with code {rc}")
-            _lib.count(int(need[0] or need[1]) + sum(need[:3]) + int(dy_img is not None))
+            _lib.count(1 + int(need[0] or need[1]) + int(dy_img is not None) + int(partial is not None))
         return dx, dwi, dwo, None
 
 

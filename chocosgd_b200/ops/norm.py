@@ -41,6 +41,11 @@ def ptr(t) -> int:
     return t.data_ptr() if t is not None else 0
 
 
+def pitch(x2: torch.Tensor) -> int:
+    """Elements from row to row of a matrix from ``rows_of`` (a single row's stride says nothing)."""
+    return x2.stride(0) if x2.shape[0] > 1 else max(1, x2.shape[1])
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -53,7 +58,7 @@ class _LayerNormFn(torch.autograd.Function):
         stats = torch.empty(2 * n, dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
         if n:
             _lib.check(_lib.packed("layer_norm_forward", "10qdq")(
-                x2.data_ptr(), x2.stride(0), ptr(weight), ptr(bias), y.data_ptr(), ptr(stats), n, d, DT[x.dtype], DT[p_dtype], eps,
+                x2.data_ptr(), pitch(x2), ptr(weight), ptr(bias), y.data_ptr(), ptr(stats), n, d, DT[x.dtype], DT[p_dtype], eps,
                 _lib.raw_stream(dev)), "layer_norm_forward")
             _lib.count(1)
         if stats is not None:
@@ -76,7 +81,7 @@ class _LayerNormFn(torch.autograd.Function):
             if need_w or need_b:
                 partial = torch.empty(_partial_floats(d), dtype=torch.float32, device=dev)
             _lib.check(_lib.packed("layer_norm_backward", "15q")(
-                x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), ptr(weight), stats.data_ptr(), ptr(dx), ptr(dw),
+                x2.data_ptr(), pitch(x2), dy2.data_ptr(), pitch(dy2), ptr(weight), stats.data_ptr(), ptr(dx), ptr(dw),
                 ptr(db), ptr(partial), n, d, DT[x2.dtype], DT[ctx.p_dtype], _lib.raw_stream(dev)), "layer_norm_backward")
             _lib.count(2 if partial is not None else 1)
         return dx, dw, db, None

@@ -155,6 +155,22 @@ def test_empty_second_derivative_and_captured_graph():
         assert torch.equal(dx, torch.autograd.grad(dropout(x, 0.5, k), x, dy)[0])
 
 
+@pytest.mark.gpu
+def test_more_than_32_bits_of_elements():
+    from chocosgd_b200.ops.dropout import dropout
+
+    n = (1 << 32) + 21                                # 8.6 GB; draws of the runs around element 2^32 and of the last ones
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    key = 0x0123456789ABCDEF
+    y = dropout(x, 0.5, torch.tensor([key], device="cuda"), site=6)
+    for run in ((1 << 29) - 1, 1 << 29, (1 << 29) + 1, n // 8):
+        want = []
+        for w in philox((run & 0xFFFFFFFF, run >> 32, 6, 0), (key & 0xFFFFFFFF, key >> 32)):
+            want += [(w & 0xFFFF) >= 32768, (w >> 16) >= 32768]
+        got = (y[run * 8:run * 8 + 8] != 0).tolist()
+        assert got == want[:len(got)], run
+
+
 def test_refusals():
     from chocosgd_b200.ops.dropout import dropout
 

@@ -165,6 +165,39 @@ def test_side_stream_and_captured_graph():
         assert torch.equal(a, r)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,dtype", [((5000, 1024), torch.bfloat16), ((2500, 4104), torch.float16), ((2400, 8192), torch.bfloat16),
+                                         ((2400, 2048), torch.float32), ((3000, 9000), torch.bfloat16), ((2401, 12000), torch.float16),
+                                         ((3000, 650), torch.float32), ((2500, 1030), torch.bfloat16), ((2400, 10240), torch.float32)])
+def test_rows_for_every_sm(shape, dtype):
+    """Enough rows for the ring of bulk copies, and widths on each side of its limits."""
+    from chocosgd_b200.ops.norm import last_error
+
+    _check(shape, dtype, dtype)
+    assert last_error() == 0
+
+
+@pytest.mark.gpu
+def test_more_than_32_bits_of_elements_single_rows_and_second_derivatives():
+    from chocosgd_b200.ops.norm import layer_norm
+
+    n, d = (1 << 21) + 3, 1024
+    x = torch.randn(1 << 10, d, device="cuda").bfloat16().repeat((1 << 11) + 1, 1)[:n].requires_grad_()
+    w = torch.randn(d, device="cuda")
+    y = layer_norm(x, w)
+    # equal rows through the same kernel give equal bits (a call with fewer rows may take another one)
+    assert torch.equal(y[-1027:-3], y[:1024]) and torch.equal(y[-3:], y[:3])
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(dx[:1024], dx[-1027:-3])
+    del y, dx, x
+    v = torch.randn(1, 64, device="cuda")
+    for stride in (0, 1, 7):
+        assert torch.equal(layer_norm(v.as_strided((1, 64), (stride, 1))), layer_norm(v))
+    v.requires_grad_()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(layer_norm(v).sum(), v, create_graph=True)
+
+
 def test_refusals():
     from chocosgd_b200.ops.norm import layer_norm, layer_norm_supported
 
