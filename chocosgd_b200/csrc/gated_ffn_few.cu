@@ -8,9 +8,11 @@
 // The lanes' sums of 32 values are brought together in 31 shuffles (each step halves the number of values a lane holds);
 // the warps of a k split meet in shared memory.  Fixed order: the same inputs give the same bits.
 //
-// Tokens: up to 8.  Above, the multiply-adds (tokens per weight) take longer than the weights' way from memory: 16-bit operands
-// then go to the tensor core; fp32, whose tensor-core form has to split the weights first, takes tiles of 32 tokens x 32 weight
-// rows on the fp32 units up to 64 tokens (ffn_tile_kernel).
+// Tokens: up to 4 for 16-bit weights, up to 8 for fp32.  Above, the multiply-adds (tokens per weight) take longer than the weights'
+// way from memory: 16-bit operands then go to the tensor core (2048 x 8192 bf16, this form against the tensor-core form: 1 token
+// 23 / 36 us, 4 tokens 33 / 37, 8 tokens 60 / 35); fp32, whose tensor-core form has to split the weights first, takes tiles of 32
+// tokens x 32 weight rows on the fp32 units up to 32 tokens (ffn_tile_kernel; 2048 x 8192: 16 tokens 123 / 165 us, 32 tokens
+// 125 / 165, 48 tokens 232 / 166).
 #include "ffn.cuh"
 #include "launch.cuh"
 
@@ -170,8 +172,11 @@ static int few_launch(FewArgs& a, cudaStream_t st) {
 template <typename TW, typename TX, typename TO, int V, bool GATE>
 static int few_tokens(FewArgs& a, cudaStream_t st) {
   if (a.m <= 1) return few_launch<TW, TX, TO, 1, V, GATE>(a, st);
+  if (a.m <= 2) return few_launch<TW, TX, TO, 2, V, GATE>(a, st);
   if (a.m <= 4) return few_launch<TW, TX, TO, 4, V, GATE>(a, st);
-  if (a.m <= 8) return few_launch<TW, TX, TO, 8, V, GATE>(a, st);
+  if constexpr (sizeof(TW) == 4) {
+    if (a.m <= 8) return few_launch<TW, TX, TO, 8, V, GATE>(a, st);
+  }
   return -1;
 }
 // V: the widest access that all rows of both factors and k allow
@@ -193,7 +198,7 @@ static int few_forward(FewArgs& in, FewArgs& out, cudaStream_t st) {
   return rc ? rc : few_width<T, float, T, false>(out, st);
 }
 
-// ---- fp32, up to 64 tokens ------------------------------------------------------------------------------------------
+// ---- fp32, 9 to 32 tokens ------------------------------------------------------------------------------------------
 // A block multiplies 32 tokens with 32 weight rows (gate: 16 gate rows and their up rows).  64 k at a time come into shared
 // memory by cp.async (four stages); four groups of 64 threads take 16 k each, a thread 4 tokens x 4 rows (8 loads of 16 bytes
 // from shared memory for 64 multiply-adds).  The groups' sums, then those of the blocks of a cluster, which share a long k
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(256) ffn_tile_kernel(FewArgs a) {
   pdl_wait();
   pdl_trigger();
   const int t = threadIdx.x, slices = a.k_split;        // blocks of a cluster
-  const int slice = (int)(blockIdx.x % slices), c0 = (int)(blockIdx.x / slices) * (GATE ? 16 : 32), m0 = blockIdx.y * 32;
+  const int slice = (int)(blockIdx.x % slices), c0 = (int)(blockIdx.x / slices) * (GATE ? 16 : 32);
   const int steps = (a.k + FT_K - 1) / FT_K;
   const int s0 = (int)((long long)steps * slice / slices), s1 = (int)((long long)steps * (slice + 1) / slices);
   const float *w = reinterpret_cast<const float*>(a.w), *x = reinterpret_cast<const float*>(a.x);
@@ -236,8 +241,8 @@ __global__ void __launch_bounds__(256) ffn_tile_kernel(FewArgs a) {
       inside = c < a.n;
       src[j] = w + (inside ? (long long)c * a.ldw + (GATE && r >= 16 ? a.up : 0) : 0) + k0;
     } else {
-      inside = m0 + r - 32 < a.m;
-      src[j] = x + (inside ? (long long)(m0 + r - 32) * a.ldx : 0) + k0;
+      inside = r - 32 < a.m;
+      src[j] = x + (inside ? (long long)(r - 32) * a.ldx : 0) + k0;
     }
     rows |= (uint32_t)inside << j;
   }
@@ -316,7 +321,7 @@ __global__ void __launch_bounds__(256) ffn_tile_kernel(FewArgs a) {
       v += p;
       u += z;
     }
-    if (c0 + r < a.n && m0 + m < a.m) {
+    if (c0 + r < a.n && m < a.m) {
       if (GATE) {
         float slope, h;
         if (a.act == ACT_SILU) h = ff_act<ACT_SILU, false, false>(v, slope);
@@ -325,7 +330,7 @@ __global__ void __launch_bounds__(256) ffn_tile_kernel(FewArgs a) {
         else h = ff_act<ACT_SIGMOID, false, false>(v, slope);
         v = h * u;
       }
-      reinterpret_cast<float*>(a.out)[(long long)(m0 + m) * a.ldo + c0 + r] = v;
+      reinterpret_cast<float*>(a.out)[(long long)m * a.ldo + c0 + r] = v;
     }
   }
   // the other blocks have read this one's sums
@@ -337,16 +342,16 @@ static int ft_launch(FewArgs& a, cudaStream_t st) {
   void (*kernel)(FewArgs) = ffn_tile_kernel<V, GATE>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FT_SMEM);
   if (e != cudaSuccess) return (int)e;
-  const int tiles = (a.n + (GATE ? 15 : 31)) / (GATE ? 16 : 32), mt = (a.m + 31) / 32, steps = (a.k + FT_K - 1) / FT_K;
+  const int tiles = (a.n + (GATE ? 15 : 31)) / (GATE ? 16 : 32), steps = (a.k + FT_K - 1) / FT_K;
   a.k_split = 1;
   // slices of k: the cheapest by  blocks per SM x (steps + what a block costs besides, about two steps)
   long long best = 1LL << 62;
   for (int q = 1; q <= 8 && q <= steps; q *= 2) {
-    const long long cost = (long long)((tiles * (long long)mt * q + sm_count() - 1) / sm_count()) * ((steps + q - 1) / q + 2);
+    const long long cost = (long long)((tiles * (long long)q + sm_count() - 1) / sm_count()) * ((steps + q - 1) / q + 2);
     if (cost < best) { best = cost; a.k_split = q; }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * a.k_split), (unsigned)mt);
+  cfg.gridDim = dim3((unsigned)(tiles * a.k_split));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = FT_SMEM;
   cfg.stream = st;
@@ -377,7 +382,7 @@ static int ft_width(FewArgs& a, cudaStream_t st) {
   return ft_launch<1, GATE>(a, st);
 }
 
-int ffn_few_tokens(int dt) { return dt == DT_F32 ? 64 : 8; }
+int ffn_few_tokens(int dt) { return dt == DT_F32 ? 32 : 4; }
 
 int ffn_few_forward(const void* x, long long ldx, const void* w_in, long long ld_in, const void* w_out, long long ld_out, float* h,
                     void* y, int m, int d, int f, int n, int act, int dt, cudaStream_t st) {
