@@ -372,7 +372,7 @@ template <int BN, int S, int KIND, int CG> struct FfnSmem {
   // Epilogue warps.  Three planes: the sums of a tile end in the epilogue's registers, so it does not run under the next tile;
   // with sixteen warps its activation and splitting take less (1120 x 650 x 2600, gate 51.8 -> 47.8 us, dgate 52.4 -> 44.8).
   // 16-bit operands: eight (dgate at 8192 x 2048 x 8192: 259 us, with sixteen and no room to fetch ahead 273).
-  static constexpr int EPI = S == 3 && (KIND == FF_DGATE || (KIND == FF_GATE && BN >= 128)) ? 16 : 8;
+  static constexpr int EPI = S == 3 && (KIND == FF_DGATE || (KIND == FF_GATE && BN >= 128) || BN == 256) ? 16 : 8;
   static constexpr int A_TILE = FF_BM * FF_BK(S) * 2, B_TILE = BN / CG * FF_BK(S) * 2;
   static constexpr int STAGE = S * (A_TILE + B_TILE);
   static constexpr int EPI_BYTES = EPI * 4096;            // 4 KB for each epilogue warp
@@ -871,13 +871,13 @@ static int ffn_launch_t(FfnBatch& batch, const FfnOperands* o, cudaStream_t st) 
 }
 
 // Which tile a launch runs with, by its time in SM cycles:  tiles per SM (pair) x (64-k blocks x step + exposed epilogue), where
-//   step      the slower of multiplying (1024 multiply-adds x 4 per cycle and SM; six times for three planes) and of fetching
-//             the operands (measured: about 58 bytes per cycle and SM from L2 when all SMs fetch)
+//   step      16-bit operands: the slower of multiplying (1024 multiply-adds x 4 per cycle and SM) and of fetching the operands
+//             (measured: about 58 bytes per cycle and SM from L2 when all SMs fetch); three planes: shared memory, from which every
+//             one of the six products reads its operands (measured about 120 bytes per cycle: 2420 cycles at a width of 128, 3200 at 256)
 //   epilogue  (measured) runs under the next tile's multiplications for 16-bit operands, not for three planes (whose sums are in
 //             the epilogue's registers)
 // One product: whole rounds.  Several: their tiles follow one another, so the average load and half of the largest tile.
-// A plain product can be cut into slices of k (not 256 wide: there the tiles are many), which costs the partial sums' second
-// pass: a launch, then 4 bytes of each written and read.
+// A plain product can be cut into slices of k, which costs the partial sums' second pass: a launch, then 4 bytes of each written and read.
 struct FfnProduct {
   int M, m_parts, cols;
   long long k64;
@@ -886,10 +886,13 @@ struct FfnPlan {
   int bn, cg, splits[3];
 };
 static double ffn_tile_cost(int bn, int cg, int S, int kind, long long k64) {
-  const double mul = 2.0 * bn * (S == 3 ? 6 : 1), fetch = S * (FF_BM + bn / cg) * 128.0 / 58.0;
-  const double main = (double)k64 * (mul > fetch ? mul : fetch);
-  double epi = bn * (kind == FF_DGATE ? 70.0 : 45.0);
-  if (S == 3) epi = kind == FF_DGATE ? 12000.0 + 110.0 * bn : (kind == FF_GATE ? 6000.0 + 30.0 * bn : 2000.0 + 90.0 * bn);
+  const double mul = 2.0 * bn, fetch = (FF_BM + bn / cg) * 128.0 / 58.0;
+  // three planes: 24 multiplications of 16 k read (128 + bn) rows of 32 bytes each from shared memory, the copies write them once
+  const double shared = (24.0 * (FF_BM + bn) * 32 + 3.0 * (FF_BM + bn / cg) * 128) / 120;
+  const double main = (double)k64 * (S == 3 ? shared : (mul > fetch ? mul : fetch));
+  // three planes, by width 64 / 128 / 256
+  static const double epi3[3][3] = {{3000, 4000, 15500}, {12000, 15500, 48000}, {6000, 10000, 19000}};
+  const double epi = S == 3 ? epi3[kind][bn == 64 ? 0 : (bn == 128 ? 1 : 2)] : bn * (kind == FF_DGATE ? 70.0 : 45.0);
   return S == 3 ? main + epi : (main > epi ? main : epi);
 }
 static FfnPlan ffn_plan(int S, int kind, const FfnProduct* p, int n) {
@@ -906,7 +909,7 @@ static FfnPlan ffn_plan(int S, int kind, const FfnProduct* p, int n) {
       total += tiles[j] * ffn_tile_cost(bn, cg, S, kind, p[j].k64);
     }
     if (low && cg == 2) continue;
-    for (int most = 1; most <= (kind == FF_PLAIN && bn < 256 ? 16 : 1); most += most < 4 ? 1 : (most < 8 ? 2 : 4)) {
+    for (int most = 1; most <= (kind == FF_PLAIN ? 16 : 1); most += most < 4 ? 1 : (most < 8 ? 2 : 4)) {
       // slices: one product `most`; several: those whose tiles are longer than 1 / most of an SM's load are cut to that
       FfnPlan plan = {bn, cg, {1, 1, 1}};
       double load = 0, largest = 0, join = 0;
