@@ -128,13 +128,14 @@ __device__ __forceinline__ void ln_get2(const float* s, int vectors, int v, F2 (
 // Rows on 16-byte boundaries, four vectors per lane.  A group (one warp up to 1024 16-bit elements) has two rows or more of its
 // own coming into shared memory by bulk copies while it works on a third in registers; the stage is filled again as soon as
 // the registers have it.  Arithmetic in pairs of fp32 numbers: one element at a time the kernel is bound by issue (18 instructions
-// per element; 16384 x 4096 bf16: 85 us, with pairs and 8 vectors per lane 77, with 4 vectors 63; 65536 x 1024: 49).
+// per element; 16384 x 4096 bf16: 85 us, with pairs and 8 vectors per lane 77, with 4 vectors 63,
+// with 768 threads 57; 65536 x 1024: 48).
 template <typename T, int NV>
-__global__ void __launch_bounds__(512, 1) ln_fwd_ring_kernel(LnArgs a, int threads, int groups, int depth) {
+__global__ void __launch_bounds__(768, 1) ln_fwd_ring_kernel(LnArgs a, int threads, int groups, int depth) {
   constexpr int V = 16 / sizeof(T);
   extern __shared__ float4 ln_smem4[];
-  __shared__ float red[16][2][32];
-  __shared__ uint64_t full[16][8];
+  __shared__ float red[24][2][32];
+  __shared__ uint64_t full[24][8];
   const int vectors = a.d / V, row_bytes = vectors * 16;
   float *w_s = reinterpret_cast<float*>(ln_smem4), *b_s = w_s + a.d;
   const int group = threadIdx.x / threads, t = threadIdx.x % threads;
@@ -616,8 +617,8 @@ template <typename T, int NV>
 static int ln_launch_fwd_ring(const LnArgs& a, cudaStream_t st, bool* done) {
   constexpr int V = 16 / sizeof(T);
   const int threads = 32 * ((a.d + 32 * V * NV - 1) / (32 * V * NV)), row_bytes = a.d * (int)sizeof(T);
-  if (threads > 512) return 0;
-  int groups = 512 / threads;
+  if (threads > 768) return 0;
+  int groups = 768 / threads;
   if (groups > 15 && threads > 32) groups = 15;
   int depth = (int)((215 * 1024 - 8LL * a.d) / ((long long)groups * row_bytes));
   if (depth > 8) depth = 8;
@@ -632,7 +633,7 @@ static int ln_launch_fwd_ring(const LnArgs& a, cudaStream_t st, bool* done) {
   return (int)launch_k(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3((unsigned)(threads * groups)), (size_t)smem, st,
                        a, threads, groups, depth);
 }
-// The ring: rows of at least 2 KB on 16-byte boundaries, enough of them for sixteen warps on every SM, room for two per group.
+// The ring: rows of at least 2 KB on 16-byte boundaries, enough of them for sixteen groups on every SM, room for two per group.
 template <typename T>
 static int ln_fwd_ring(const LnArgs& a, cudaStream_t st, bool* done) {
   *done = false;
