@@ -10,6 +10,7 @@
 // Bound by memory: one 32-bit word per element would make it issue-bound (128 Mi bf16 elements, 2 x 256 MB: 113 us
 // against 84.1 us with 16-bit draws and 83.8 us for the same loop without a generator).  Four independent 16-byte
 // runs per thread and iteration keep enough loads in flight.
+#include "block_calls.h"
 #include "launch.cuh"
 #include "vec.cuh"
 
@@ -122,22 +123,12 @@ static int dropout_launch(const void* x, const void* res, void* y, long long n, 
                               : launch_k(dropout_kernel<T, 1, false>, g, b, 0, st, px, pr, py, n, k, site, drop, scale));
 }
 
-// y[i] = res[i] + keep(i) x[i] 65536 / (65536 - drop), i < n; res may be null; key: 8 bytes on the device;
-// drop = 0 .. 65535 (65536, everything dropped, is the caller's).  The call takes one struct of 8-byte members.
-struct DropoutCall {
-  const void *x, *res;
-  void* y;
-  long long n;
-  const void* key;
-  long long site, drop, dt;
-  cudaStream_t stream;
-};
 extern "C" int dropout_apply(const DropoutCall* c) {
   if (c->n <= 0 || c->drop < 0 || c->drop > 65535 || ((uintptr_t)c->key & 3) != 0) return -1;
   const float scale = 65536.f / (65536.f - (float)c->drop);
   const uint32_t site = (uint32_t)c->site, drop = (uint32_t)c->drop;
-  if (c->dt == DT_F32) return dropout_launch<float>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, c->stream);
-  if (c->dt == DT_BF16) return dropout_launch<__nv_bfloat16>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, c->stream);
-  if (c->dt == DT_F16) return dropout_launch<__half>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, c->stream);
+  if (c->dt == DT_F32) return dropout_launch<float>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, (cudaStream_t)c->stream);
+  if (c->dt == DT_BF16) return dropout_launch<__nv_bfloat16>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, (cudaStream_t)c->stream);
+  if (c->dt == DT_F16) return dropout_launch<__half>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, (cudaStream_t)c->stream);
   return -1;
 }

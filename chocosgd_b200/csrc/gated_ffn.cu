@@ -28,6 +28,7 @@
 // accumulator 8.5e-7, and 5 % less time).
 //
 // Every mbarrier wait is bounded; a wait that runs out sets the error word, the CTA drains and frees its TMEM.
+#include "block_calls.h"
 #include "launch.cuh"
 #include "tc_common.cuh"
 #include "ffn.cuh"
@@ -1060,32 +1061,13 @@ extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt
 // most tokens of an evaluation pass that the form for few tokens takes (`few` of gated_ffn_forward)
 extern "C" int gated_ffn_few_tokens(int dt) { return ffn_few_tokens(dt); }
 
-// few: no operand images, no partial sums and no z; h: m x pad16(f) fp32.  Else:
-// Every operand comes with an optional image: [S][rows][pad16(cols)] 16-bit elements, S = 3 for fp32, needed for fp32 and
-// for rows that do not start on 16-byte boundaries.  h: [S][m][pad16(f)] 16-bit; z: 2 x (m rounded up to 32) x pad16(f) fp32 or null;
-// partial: gated_ffn_partial_floats.
-struct FfnForwardCall {          // the calls take one struct of 8-byte members
-  const void* x;
-  long long ldx;
-  void* x_img;
-  const void* w_in;
-  long long ld_in;
-  void* in_img;
-  const void* w_out;
-  long long ld_out;
-  void *out_img, *h;
-  float *z, *partial;
-  void* y;
-  long long m, d, f, n, act, dt, few;
-  cudaStream_t st;
-};
 extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
   const void *x = c->x, *w_in = c->w_in, *w_out = c->w_out;
   void *x_img = c->x_img, *in_img = c->in_img, *out_img = c->out_img, *h = c->h, *y = c->y;
   float *z = c->z, *partial = c->partial;
   const long long ldx = c->ldx, ld_in = c->ld_in, ld_out = c->ld_out;
   const int m = (int)c->m, d = (int)c->d, f = (int)c->f, n = (int)c->n, act = (int)c->act, dt = (int)c->dt;
-  const cudaStream_t st = c->st;
+  const cudaStream_t st = (cudaStream_t)c->st;
   const FfnShape s = {m, d, f, n, act, dt};
   if (!ffn_shape_ok(s)) return -1;
   if (c->few) return ffn_few_forward(x, ldx, w_in, ld_in, w_out, ld_out, reinterpret_cast<float*>(h), y, m, d, f, n, act, dt, st);
@@ -1119,29 +1101,6 @@ extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
   return ffn_plain(S, ffn_plan(S, FF_PLAIN, &p, 1), batch, &index, &o, dt, partial, st);
 }
 
-// x, w_in, w_out: as in the forward pass; where an image is given it holds the forward pass' image already.
-// dz: [S][2][m][pad16(f)] 16-bit scratch.  dx, dw_in, dw_out may be null.
-struct FfnBackwardCall {
-  const void* x;
-  long long ldx;
-  void* x_img;
-  const void* w_in;
-  long long ld_in;
-  void* in_img;
-  const void* w_out;
-  long long ld_out;
-  void* out_img;
-  const void* dy;
-  long long ldy;
-  void* dy_img;
-  const void* h;
-  float* z;
-  void* dz;
-  float* partial;
-  void *dx, *dw_in, *dw_out;
-  long long m, d, f, n, act, dt;
-  cudaStream_t st;
-};
 extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
   const void *x = c->x, *w_in = c->w_in, *w_out = c->w_out, *dy = c->dy, *h = c->h;
   void *x_img = c->x_img, *in_img = c->in_img, *out_img = c->out_img, *dy_img = c->dy_img, *dz = c->dz;
@@ -1149,7 +1108,7 @@ extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
   float *z = c->z, *partial = c->partial;
   const long long ldx = c->ldx, ld_in = c->ld_in, ld_out = c->ld_out, ldy = c->ldy;
   const int m = (int)c->m, d = (int)c->d, f = (int)c->f, n = (int)c->n, act = (int)c->act, dt = (int)c->dt;
-  const cudaStream_t st = c->st;
+  const cudaStream_t st = (cudaStream_t)c->st;
   const FfnShape s = {m, d, f, n, act, dt};
   if (!ffn_shape_ok(s)) return -1;
   const int S = dt == DT_F32 ? 3 : 1;

@@ -17,6 +17,7 @@
 //
 // Rows that do not start on 16-byte boundaries take narrower accesses (V elements at a time); rows too long for registers
 // (above 16384 elements) take the *_long kernels, which read the row again from L2.
+#include "block_calls.h"
 #include "launch.cuh"
 #include "tc_common.cuh"
 #include "vec.cuh"
@@ -729,18 +730,6 @@ static int ln_run(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStream_t s
   return -1;
 }
 
-// The calls take one struct of 8-byte members.
-// y = layer_norm(x) w + b; stats: mean [n] and 1 / sqrt(var + eps) [n], or null (evaluation)
-struct LnForwardCall {
-  const void* x;
-  long long ldx;
-  const void *w, *b;
-  void* y;
-  float* stats;
-  long long n, d, dt, w_dt;
-  double eps;
-  cudaStream_t stream;
-};
 extern "C" int layer_norm_forward(const LnForwardCall* c) {
   LnArgs a = {};
   a.x = c->x; a.w = c->w; a.b = c->b; a.y = c->y; a.n = c->n; a.ldx = c->ldx; a.d = (int)c->d; a.eps = (float)c->eps;
@@ -748,31 +737,18 @@ extern "C" int layer_norm_forward(const LnForwardCall* c) {
   a.mean = c->stats;
   a.rstd = c->stats != nullptr ? c->stats + c->n : nullptr;
   int blocks = 0;
-  return ln_run(a, (int)c->dt, false, &blocks, c->stream);
+  return ln_run(a, (int)c->dt, false, &blocks, (cudaStream_t)c->stream);
 }
 
-// dx (may be null) and dw, db (may be null; partial: layer_norm_partial_floats(d) floats of scratch, or null without both)
-struct LnBackwardCall {
-  const void* x;
-  long long ldx;
-  const void* dy;
-  long long lddy;
-  const void* w;
-  float* stats;
-  void *dx, *dw, *db;
-  float* partial;
-  long long n, d, dt, w_dt;
-  cudaStream_t stream;
-};
 extern "C" int layer_norm_backward(const LnBackwardCall* c) {
   if ((c->dw != nullptr || c->db != nullptr) != (c->partial != nullptr)) return -1;
   LnArgs a = {};
   a.x = c->x; a.dy = c->dy; a.lddy = c->lddy; a.w = c->w; a.mean = c->stats; a.rstd = c->stats + c->n;
   a.dx = c->dx; a.partial = c->partial; a.n = c->n; a.ldx = c->ldx; a.d = (int)c->d; a.w_dt = (int)c->w_dt;
   int blocks = 0;
-  const int rc = ln_run(a, (int)c->dt, true, &blocks, c->stream);
+  const int rc = ln_run(a, (int)c->dt, true, &blocks, (cudaStream_t)c->stream);
   if (rc || c->partial == nullptr) return rc;
-  return (int)launch_k(ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, c->stream,
+  return (int)launch_k(ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, (cudaStream_t)c->stream,
                        (const float*)c->partial, blocks, a.d, c->dw, c->db, a.w_dt);
 }
 

@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 from ctypes import POINTER, Structure, c_float, c_int, c_int32, c_longlong, c_uint32, c_void_p
 
 _LIB = None
@@ -67,13 +66,24 @@ def check(code: int, what: str = ""):
 
 MAX_PEERS = 16
 
+
+class _Launches:
+    """``LAUNCHES[0]``: launches counted here and by the autograd nodes."""
+
+    def __init__(self):
+        self.own = 0
+
+    def __getitem__(self, i):
+        return self.own + (_NODES.launches() if _NODES is not None else 0)
+
+
 #: kernels of this library launched so far by this process (the Python wrappers add their
 #: launches; a training step captured in a CUDA graph replays the count taken while capturing)
-LAUNCHES = [0]
+LAUNCHES = _Launches()
 
 
 def count(n: int = 1):
-    LAUNCHES[0] += n
+    LAUNCHES.own += n
 
 
 class SegTableC(Structure):
@@ -221,43 +231,23 @@ def ptr(t):
     return c_void_p(t.data_ptr()) if t is not None else c_void_p(0)
 
 
-def on_device(device, fn, *args):
-    """``fn(*args)`` with ``device`` as the current device (kernels and their streams are the current device's)."""
-    import torch
-
-    if device.index is None or device.index == torch.cuda.current_device():
-        return fn(*args)
-    with torch.cuda.device(device):
-        return fn(*args)
+_NODES = None
 
 
-_PACKED = {}
+def nodes():
+    """The module of autograd nodes (``csrc/autograd.cpp``): layer_norm, dropout, gated_ffn."""
+    global _NODES
+    if _NODES is None:
+        import importlib.util
 
+        import torch  # noqa: F401  (its libraries have to be in the process before the module is)
 
-def packed(name: str, fmt: str):
-    """The entry point ``name``, which takes one pointer to a struct of 8-byte members (``fmt``: ``q`` pointers and integers,
-    ``d`` floating numbers), as a function of the members that returns the error code.  One ``struct.pack`` costs a fraction of
-    converting twenty arguments one by one, which would be a third of the host time of a small call."""
-    call = _PACKED.get(name)
-    if call is None:
-        fn = getattr(load(), name)
-        fn.argtypes, fn.restype = [ctypes.c_char_p], c_int
-        pack = struct.Struct("=" + fmt).pack
-        call = _PACKED[name] = lambda *members: fn(pack(*members))
-    return call
-
-
-def raw_stream(device) -> int:
-    """``cudaStream_t`` of the current stream of ``device`` as an integer."""
-    import torch
-
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(device.index) if get is not None else torch.cuda.current_stream(device).cuda_stream
-
-
-def no_second_derivative(what: str):
-    """Raised in a backward pass that is itself being recorded (``create_graph=True``)."""
-    import torch
-
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what}: the backward kernels have no derivative (create_graph=True)")
+        load()
+        path = os.path.join(os.path.dirname(lib_path()), "_choco_autograd.so")
+        spec = importlib.util.spec_from_file_location("_choco_autograd", path)
+        if spec is None or not os.path.exists(path):
+            raise RuntimeError(f"native module {path} is missing: run python -m chocosgd_b200.build_ext")
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _NODES = module
+    return _NODES
