@@ -227,7 +227,7 @@ Tensor bytes(long long n, const Tensor& like) { return at::empty({n}, like.optio
 
 Tensor ffn_run(const Tensor& x, const Tensor& x2, const Tensor& wi, const Tensor& wo, int64_t act, bool train, Tensor* kept) {
   const int m = (int)x2.size(0), d = (int)x2.size(1), f = (int)wo.size(1), n = (int)wo.size(0), dt = dtype_code(x.scalar_type());
-  const bool few = !train && m <= gated_ffn_few_tokens(dt);
+  const bool few = !train && gated_ffn_few(m, d, f, n, dt);
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = n;
   Tensor y = empty(shape, x), partial;

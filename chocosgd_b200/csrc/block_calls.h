@@ -89,7 +89,7 @@ long long layer_norm_partial_floats(int d);
 int dropout_apply(const DropoutCall* c);
 int gated_ffn_forward(const FfnForwardCall* c);
 int gated_ffn_backward(const FfnBackwardCall* c);
-int gated_ffn_few_tokens(int dt);
+int gated_ffn_few(int m, int d, int f, int n, int dt);
 long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt, int backward);
 const char* choco_cuda_error_string(int code);
 }

@@ -193,26 +193,6 @@ __device__ __forceinline__ void st32b(void* p, const uint32_t* r) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
-__device__ __forceinline__ uint32_t pack2(float a, float b, int fp16) {
-  if (fp16) {
-    const __half2 q = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&q);
-  }
-  const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&q);
-}
-
-// two fp32 numbers as three pairs of bf16 numbers, each the rounded remainder of the ones before.  The first is limited to
-// the largest bf16 number, so that fp32 numbers above it keep a finite split; non-finite numbers stay non-finite.
-__device__ __forceinline__ void split3(float x, float y, uint32_t (&q)[3]) {
-  const float big = __uint_as_float(0x7F7F0000u);
-#pragma unroll
-  for (int s = 0; s < 3; ++s) {
-    q[s] = s == 0 ? pack2(fminf(fmaxf(x, -big), big), fminf(fmaxf(y, -big), big), 0) : pack2(x, y, 0);
-    x -= __uint_as_float(q[s] << 16);
-    y -= __uint_as_float(q[s] & 0xFFFF0000u);
-  }
-}
 
 // ---- a warp's 32 rows x up to 128 bytes through shared memory, so that rows are written as whole lines -----------------
 // 16-byte unit c of row r lies at unit c ^ (r & 7) of the row's 128 bytes
@@ -1058,8 +1038,8 @@ extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt
   return ffn_partial_floats(ffn_plan(S, FF_PLAIN, p, backward ? 3 : 1), p, backward ? 3 : 1);
 }
 
-// most tokens of an evaluation pass that the form for few tokens takes (`few` of gated_ffn_forward)
-extern "C" int gated_ffn_few_tokens(int dt) { return ffn_few_tokens(dt); }
+// whether an evaluation pass takes the form for few tokens (`few` of gated_ffn_forward)
+extern "C" int gated_ffn_few(int m, int d, int f, int n, int dt) { return ffn_few_fits(m, d, f, n, dt); }
 
 extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
   const void *x = c->x, *w_in = c->w_in, *w_out = c->w_out;

@@ -156,6 +156,14 @@ def test_few_tokens(m, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,d,f,n", [(12, 4096, 24, 40), (16, 40, 4100, 24), (30, 2002, 31, 33), (13, 1, 1, 1), (16, 31, 700, 650), (9, 650, 2600, 650)])
+def test_few_tokens_long_and_short_sums(m, d, f, n, dtype):
+    """One block or a cluster of eight for the sum over k, less than a step of it, rows that fill no tile."""
+    _check(m, d, f, n, dtype, "gelu")
+
+
+@pytest.mark.gpu
 def test_leading_dimensions_strides_and_broadcast_gradients():
     from chocosgd_b200.ops.ffn import gated_ffn
 
