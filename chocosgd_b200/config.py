@@ -283,7 +283,7 @@ def build_parser() -> argparse.ArgumentParser:
                    "backward pass, never stored (other masks from the same seed)")
     p.add_argument("--native_layers", default="auto", choices=("auto", "all", "off", "bn", "conv"),
                    help="layers routed to the hand-written sm_100a kernels on CUDA: auto = batch-norm + 3x3 "
-                   "convolution fwd/dgrad/wgrad, all = auto + linear + LSTM cell, "
+                   "convolution fwd/dgrad/wgrad, layer norm, gated feed-forward, all = auto + linear + LSTM cell, "
                    "bn = batch-norm + linear only, conv = bn + convolution fwd/dgrad, off = library ops")
     p.add_argument("--overlap_gossip", default=True, type=str2bool)
     p.add_argument("--qsgd_levels", default=None, type=int,

@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -129,7 +130,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps) {
   Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
   if (!layer_norm_ok(x, w, b))
     throw pybind11::value_error(
@@ -178,7 +179,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
 };
 
 // drop: the probability in steps of 2^-16, 0 .. 65535
-Tensor dropout(const Tensor& x, int64_t drop, const Tensor& key, int64_t site, const std::optional<Tensor>& res) {
+Tensor dropout(const Tensor& x, int64_t drop, const Tensor& key, int64_t site, const Maybe& res) {
   const Tensor residual = res.value_or(Tensor());
   if (!x.is_cuda() || dtype_code(x.scalar_type()) < 0)
     throw pybind11::value_error("dropout: needs a CUDA tensor of fp32, bf16 or fp16, got " + describe(x));
@@ -330,12 +331,13 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("layer_norm", &layer_norm);
-  m.def("layer_norm_supported", [](const Tensor& x, const std::optional<Tensor>& w, const std::optional<Tensor>& b) {
+  // wrapped: an allocation that fails raises PyTorch's own exception
+  m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
+  m.def("layer_norm_supported", [](const Tensor& x, const Maybe& w, const Maybe& b) {
     return layer_norm_ok(x, w.value_or(Tensor()), b.value_or(Tensor()));
   });
-  m.def("dropout", &dropout);
-  m.def("gated_ffn", &gated_ffn);
+  m.def("dropout", torch::wrap_pybind_function(dropout));
+  m.def("gated_ffn", torch::wrap_pybind_function(gated_ffn));
   m.def("gated_ffn_supported", &gated_ffn_ok);
   m.def("launches", []() { return g_launches.load(); });
 }

@@ -24,8 +24,13 @@
 // it.  The tensor core truncates when it adds to its accumulator, which over a long K costs far more than that
 // (measured, one pass of exactly representable operands: relative error 7e-8 at K = 64, 4.4e-6 at K = 2600), so the fp32
 // form takes its accumulator out after every 32 k and adds it up in registers; within those the small products go first.
-// The whole operator at 1120 x 650 x 2600: 2.7e-7 off 64 bits, the same in fp32 arithmetic 9e-7 to 1.5e-6 (with 64 k per
+// The whole operator at 1120 x 650 x 2600: 2.5e-7 off 64 bits, the same in fp32 arithmetic 9e-7 to 1.5e-6 (with 64 k per
 // accumulator 8.5e-7, and 5 % less time).
+//
+// Bound by the tensor cores: 8192 x 2048 x 8192 bf16, gate 403 us (1.36 PFLOP/s), Y 191 (1.44), dgate 253 (1.09: it reads 0.5 GB
+// of G and U and writes 0.27 GB), the three gradient products 924 (1.49); the library's plain products of the same sizes take 352,
+// 178, 175 and 882 us without activation, G, U or their gradients.  fp32, 1120 x 650 x 2600: gate 52 us, Y 33 + 6, dgate 48, the
+// gradients 125 + 8, images 16; there the epilogue, which takes the accumulator out every 32 k, costs as much as the products.
 //
 // Every mbarrier wait is bounded; a wait that runs out sets the error word, the CTA drains and frees its TMEM.
 #include "block_calls.h"

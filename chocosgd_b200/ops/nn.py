@@ -42,8 +42,9 @@ AUTO_KINDS = ("bn", "conv", "wgrad", "ce", "linear", "pool", "embed", "norm", "f
 
 def configure_native(mode: str = "auto"):
     """Apply a ``--native_layers`` choice: auto = batch-norm + 3x3 convolution forward / input /
-    weight gradient, all = every kind built into the tree, bn = batch-norm + linear, conv = bn +
-    convolution forward / input gradient, off = library ops only."""
+    weight gradient, large linear layers, layer norm, gated feed-forward, all = every kind built
+    into the tree, bn = batch-norm + linear, conv = bn + convolution forward / input gradient,
+    off = library ops only."""
     set_native(False, which=tuple(_NATIVE))
     if mode in ("off", None) or not torch.cuda.is_available():
         return
@@ -161,7 +162,7 @@ class Dropout(nn.Dropout):
             from .dropout import dropout, dropout_supported, new_key
 
             if dropout_supported(x):
-                if residual is not None and residual.dtype != x.dtype:
+                if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
                     return residual + dropout(x, self.p, new_key(x.device))
                 return dropout(x, self.p, new_key(x.device), residual=residual)
         y = super().forward(x)

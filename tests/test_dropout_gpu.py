@@ -191,3 +191,18 @@ def test_refusals_on_the_device():
                      ((x, 0.5, k), {"residual": x[:2]}), ((x, 0.5, k), {"residual": x.half()}), ((x, 0.5, k), {"residual": x.cpu()})):
         with pytest.raises(ValueError):
             dropout(*args, **kw)
+
+
+@pytest.mark.gpu
+def test_layer_with_a_residual_of_another_shape_or_type():
+    from chocosgd_b200.ops.nn import Dropout, set_native
+
+    x, bias = torch.ones(64, 96, device="cuda"), torch.full((96,), 3.0, device="cuda")
+    layer = Dropout(0.5)
+    try:
+        set_native(True, which=("dropout",))
+        for r in (bias, torch.full((64, 96), 3.0, device="cuda", dtype=torch.bfloat16)):
+            y = layer(x, r)
+            assert y.shape == x.shape and set(y.unique().tolist()) == {3.0, 5.0}
+    finally:
+        set_native(False, which=("dropout",))

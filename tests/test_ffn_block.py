@@ -214,3 +214,85 @@ def test_training_step_of_the_model_with_the_block(native):
     assert (x_e - x_g).abs().max() < 1e-3 * x_e.abs().max()
     losses, _ = run(native, True, "0.5")                     # with masks: every replay draws its own
     assert all(l == l for l in losses) and len(set(losses)) == 3
+
+
+def _block(x, w, b, wi, wo, key, p=0.25):
+    from chocosgd_b200.ops.dropout import dropout
+    from chocosgd_b200.ops.ffn import gated_ffn
+    from chocosgd_b200.ops.norm import layer_norm
+
+    return dropout(gated_ffn(layer_norm(x, w, b), wi, wo), p, key, site=2, residual=x)
+
+
+def _block_inputs(rows, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    dim, hidden = 136, 272
+    shapes = ((rows, dim), (dim,), (dim,), (2 * hidden, dim), (dim, hidden))
+    leaves = [torch.randn(*s, device="cuda", generator=g).mul_(0.3).to(dtype).requires_grad_() for s in shapes]
+    return leaves, torch.randn(rows, dim, device="cuda", generator=g).to(dtype), torch.tensor([seed * 7919 + 1], device="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_graph_that_is_kept_gives_the_same_gradients_again(dtype):
+    leaves, dy, key = _block_inputs(150, dtype, 1)
+    y = _block(*leaves, key)
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    for p, q in zip(first, torch.autograd.grad(y, leaves, dy)):
+        assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_parameters_changed_in_place_are_refused_in_the_backward_pass():
+    for which in range(1, 5):
+        if which == 2:
+            continue                                        # the bias is no part of any derivative
+        leaves, dy, key = _block_inputs(9, torch.float32, 2)
+        y = _block(*leaves, key)
+        with torch.no_grad():
+            leaves[which].mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.gpu
+def test_two_threads_on_streams_of_their_own():
+    """Forward and backward passes of two threads at once, of different sizes and types: each as if it were alone."""
+    import threading
+
+    work = [_block_inputs(150, torch.float32, 3), _block_inputs(70, torch.bfloat16, 4)]
+    alone = [torch.autograd.grad(_block(*leaves, key), leaves, dy) for leaves, dy, key in work]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                leaves, dy, key = work[i]
+                for _ in range(20):
+                    got[i] = torch.autograd.grad(_block(*leaves, key), leaves, dy)
+        except Exception as e:                              # reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for a, b in zip(alone, got):
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_launches_of_the_nodes_are_counted():
+    from chocosgd_b200.ops import _lib
+
+    leaves, dy, key = _block_inputs(40, torch.bfloat16, 5)
+    n0 = _lib.LAUNCHES[0]
+    y = _block(*leaves, key)
+    n1 = _lib.LAUNCHES[0]
+    torch.autograd.grad(y, leaves, dy)
+    assert n1 - n0 >= 4 and _lib.LAUNCHES[0] - n1 >= 5      # norm, gate, output, dropout; their gradients

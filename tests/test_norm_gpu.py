@@ -218,3 +218,14 @@ def test_refusals_on_the_device():
                  (x[:, :0],)):
         with pytest.raises(ValueError):
             layer_norm(*args)
+
+
+@pytest.mark.gpu
+def test_allocation_failure_is_pytorchs_exception():
+    """An expanded input whose copy (a tebibyte) no device holds: the error is the one that callers catch, and the next call works."""
+    from chocosgd_b200.ops.norm import layer_norm
+
+    row = torch.ones(1, 1024, device="cuda")
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        layer_norm(row.expand(1 << 28, 1024))
+    assert torch.equal(layer_norm(row.expand(3, 1024)), torch.zeros(3, 1024, device="cuda"))
