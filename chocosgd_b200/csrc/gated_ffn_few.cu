@@ -8,10 +8,10 @@
 // sums, h in fp32.  The lanes' sums of 32 values are brought together in 31 shuffles (each step halves the number of values a lane
 // holds); the warps of a k split meet in shared memory.  Fixed order: the same inputs give the same bits.
 //
-// Above, the multiply-adds (tokens per weight) take longer than the weights' way from memory (2048 x 8192 bf16: 1 token 23 us,
+// Above, the multiply-adds (tokens per weight) take longer than the weights' way from memory (2048 x 8192 bf16: 1 token 22 us,
 // 4 tokens 33, 8 tokens 60), and the products go to the warps' matrix instruction (ffn_mma_kernel): fp32 up to 32 tokens, which
-// saves the tensor-core form's pass that splits the weights (32 tokens, this form / that one: 650 x 2600 27 / 39 us, 2048 x 8192
-// 95 / 166; 48 tokens 43 / 39 and 195 / 166); 16 bits up to 16 tokens and 2^25 weights, where that form's setup counts
+// saves the tensor-core form's pass that splits the weights (32 tokens, this form / that one: 650 x 2600 26 / 39 us, 2048 x 8192
+// 93 / 166; 48 tokens 43 / 39 and 195 / 166); 16 bits up to 16 tokens and 2^25 weights, where that form's setup counts
 // (16 tokens: 650 x 2600 14 / 21, 1536 x 6144 25 / 29, 2048 x 8192 39 / 36; 32 tokens: 20 / 21, 32 / 28, 53 / 32).
 #include "ffn.cuh"
 #include "launch.cuh"
@@ -83,8 +83,6 @@ __global__ void __launch_bounds__(FEW_THREADS) ffn_few_kernel(FewArgs a) {
   constexpr int RG = GATE ? FEW_ROWS / 2 : FEW_ROWS;     // result columns of a warp
   constexpr int NV = FEW_ROWS * MT;
   __shared__ float sums[2][FEW_WARPS][NV];
-  pdl_wait();
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ks = warp & (a.k_split - 1), group = warp / a.k_split, groups = FEW_WARPS / a.k_split;
   const int all = (a.n + RG - 1) / RG;       // groups of result columns, dealt out to the blocks
@@ -94,6 +92,8 @@ __global__ void __launch_bounds__(FEW_THREADS) ffn_few_kernel(FewArgs a) {
   const int s0 = (int)((long long)steps * ks / a.k_split), s1 = (int)((long long)steps * (ks + 1) / a.k_split);
   const TW* w = reinterpret_cast<const TW*>(a.w);
   const TX* x = reinterpret_cast<const TX*>(a.x);
+  pdl_wait();
+  pdl_trigger();
   int turn = 0;
   for (int base = c0; base < c1; base += RG * groups, turn ^= 1) {
     const int col = base + group * RG;
@@ -152,6 +152,8 @@ __global__ void __launch_bounds__(FEW_THREADS) ffn_few_kernel(FewArgs a) {
   }
 }
 
+// The second product is always launched as a programmatic dependent of the first (1 token, 2048 x 8192 bf16: 23.2 -> 21.9 us;
+// with its weights prefetched into L2 before its wait 22.6).
 // Blocks: as many as fit on an SM by their registers (four, two), fewer for few columns.  Warps per row (k_split): the
 // cheapest by  rounds of a block x (steps x cycles of a step + cycles of bringing the sums together), with two to eight warps
 // on a scheduler.
@@ -168,7 +170,7 @@ static int few_launch(FewArgs& a, cudaStream_t st) {
     const long long cost = (long long)((groups + wr - 1) / wr) * ((long long)((steps + q - 1) / q) * step + join);
     if (cost < best) { best = cost; a.k_split = q; }
   }
-  return (int)launch_k(ffn_few_kernel<TW, TX, TO, MT, V, GATE>, dim3(grid), dim3(FEW_THREADS), 0, st, a);
+  return (int)launch_k_if(!GATE || pdl_enabled(), ffn_few_kernel<TW, TX, TO, MT, V, GATE>, dim3(grid), dim3(FEW_THREADS), 0, st, a);
 }
 // ---- more tokens: the warps' matrix instruction ------------------------------------------------------------------------
 // A block multiplies 32 tokens (8 NT) with 32 weight rows (gate: 16 gate rows and their up rows, which meet in one thread); its
@@ -178,7 +180,7 @@ static int few_launch(FewArgs& a, cudaStream_t st) {
 // into three bf16 parts in registers (six products, the small ones first) and the instruction's sum, which is truncated, is added
 // to the fp32 one after every step.  The warps' sums, then those of the cluster, are added in a fixed order.  Bound by the
 // latency of a step (loads, splitting, 96 matrix instructions; eight warps per SM by their registers): 32 tokens fp32, 650 x
-// 2600, 27 us for 20 MB of weights (the same tile on the fp32 units, fed through shared memory: 31; 2048 x 8192: 125, here 95).
+// 2600, 26 us for 20 MB of weights (the same tile on the fp32 units, fed through shared memory: 31; 2048 x 8192: 125, here 93).
 #define FM_WARPS 4
 #define FM_MI 2                      // instructions' rows of a warp: 2 x 16 (one: 2048 x 8192 fp32, 16 tokens 97 us, two 79)
 #define FM_ROWS (16 * FM_MI)
@@ -237,7 +239,8 @@ __device__ __forceinline__ void fm_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// blocks that an SM holds by their registers
+// blocks that an SM holds by their registers (fp32, 32 tokens, three with the tokens' loads one instruction ahead only: 31 against
+// 26 us, 2048 x 8192 141 against 93)
 template <typename TW, int NT>
 constexpr int fm_resident() { return sizeof(TW) == 4 && NT == 4 ? 2 : 3; }
 
@@ -269,7 +272,8 @@ __global__ void __launch_bounds__(32 * FM_WARPS, (fm_resident<TW, NT>())) ffn_mm
 #pragma unroll
       for (int h = 0; h < 2; ++h) fm_load<TW, V>(w[i][h] + s * 32, a.k - s * 32 - k0, rw[i][h]);
   };
-  // the second product's weights need not wait for the first product: whoever wrote them was waited for by that one
+  // the second product's weights need not wait for the first product: that kernel triggers this one's launch only after its own
+  // wait, so whoever wrote them has completed
   if (!GATE && s0 < s1) load_w(s0);
   pdl_wait();
   pdl_trigger();
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(32 * FM_WARPS, (fm_resident<TW, NT>())) ffn_mm
       uint32_t q[S][4];
       fm_parts<TW, TX, S>(rx[j], q);
       if (s + 1 < s1) fm_load<TX, VX>(x[j] + (s + 1) * 32, a.k - (s + 1) * 32 - k0, rx[j]);
-      float c[FM_MI][4] = {};
+      float c[FM_MI][2][4] = {};             // a sum for each half of the step: more independent instructions
 #pragma unroll
       for (int o = S - 1; o >= 0; --o)       // parts u of the weight and o - u of the token
 #pragma unroll
@@ -301,11 +305,11 @@ __global__ void __launch_bounds__(32 * FM_WARPS, (fm_resident<TW, NT>())) ffn_mm
           for (int e = 0; e < 4; e += 2)
 #pragma unroll
             for (int i = 0; i < FM_MI; ++i)
-              fm_mma<HALF>(c[i], p[i][0][u][e], p[i][1][u][e], p[i][0][u][e + 1], p[i][1][u][e + 1], q[o - u][e], q[o - u][e + 1]);
+              fm_mma<HALF>(c[i][e / 2], p[i][0][u][e], p[i][1][u][e], p[i][0][u][e + 1], p[i][1][u][e + 1], q[o - u][e], q[o - u][e + 1]);
 #pragma unroll
       for (int i = 0; i < FM_MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] += c[i][e];
+        for (int e = 0; e < 4; ++e) acc[i][j][e] += c[i][0][e] + c[i][1][e];
     }
   }
   // sums [warp][row][token]; gate: rows 0 .. 15 the gate's, 16 .. 31 the up rows'
@@ -378,7 +382,7 @@ static int fm_launch(FewArgs& a, cudaStream_t st) {
     at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (pdl_enabled()) {
+  if (!GATE || pdl_enabled()) {
     at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;

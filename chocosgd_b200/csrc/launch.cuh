@@ -6,7 +6,8 @@
 // allocation), and block in pdl_wait() until the previous kernel has completed and its writes
 // are visible.  Rules followed by every kernel in this library that is launched this way:
 //   * pdl_wait() is executed unconditionally by every CTA before its first access to global
-//     memory (so completion stays transitive along the stream);
+//     memory (so completion stays transitive along the stream; the one exception, which gated_ffn_few.cu explains, reads inputs
+//     that the kernel before it in the same call has waited for);
 //   * nothing is written to global memory before pdl_wait().
 // Inside a captured CUDA graph the attribute becomes a programmatic dependency edge.  Without the
 // attribute (the default, or a launch by plain <<<>>>) both calls are no-ops.
@@ -49,8 +50,8 @@ static inline bool pdl_enabled() {
 }
 
 template <typename... P, typename... A>
-static inline cudaError_t launch_k(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                                   A&&... args) {
+static inline cudaError_t launch_k_if(bool pdl, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                      A&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -60,6 +61,11 @@ static inline cudaError_t launch_k(void (*kernel)(P...), dim3 grid, dim3 block, 
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+template <typename... P, typename... A>
+static inline cudaError_t launch_k(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                   A&&... args) {
+  return launch_k_if(pdl_enabled(), kernel, grid, block, smem, st, std::forward<A>(args)...);
 }
