@@ -272,13 +272,10 @@ __global__ void __launch_bounds__(32 * FM_WARPS, (fm_resident<TW, NT>())) ffn_mm
 #pragma unroll
       for (int h = 0; h < 2; ++h) fm_load<TW, V>(w[i][h] + s * 32, a.k - s * 32 - k0, rw[i][h]);
   };
-  // the second product's weights need not wait for the first product: that kernel triggers this one's launch only after its own
-  // wait, so whoever wrote them has completed
-  if (!GATE && s0 < s1) load_w(s0);
   pdl_wait();
   pdl_trigger();
   if (s0 < s1) {
-    if (GATE) load_w(s0);
+    load_w(s0);
 #pragma unroll
     for (int j = 0; j < NT; ++j) fm_load<TX, VX>(x[j] + s0 * 32, a.k - s0 * 32 - k0, rx[j]);
   }

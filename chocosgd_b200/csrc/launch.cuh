@@ -6,8 +6,7 @@
 // allocation), and block in pdl_wait() until the previous kernel has completed and its writes
 // are visible.  Rules followed by every kernel in this library that is launched this way:
 //   * pdl_wait() is executed unconditionally by every CTA before its first access to global
-//     memory (so completion stays transitive along the stream; the one exception, which gated_ffn_few.cu explains, reads inputs
-//     that the kernel before it in the same call has waited for);
+//     memory (so completion stays transitive along the stream);
 //   * nothing is written to global memory before pdl_wait().
 // Inside a captured CUDA graph the attribute becomes a programmatic dependency edge.  Without the
 // attribute (the default, or a launch by plain <<<>>>) both calls are no-ops.
