@@ -164,6 +164,52 @@ def test_few_tokens_long_and_short_sums(m, d, f, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [2, 7, 12, 24])
+def test_few_tokens_in_graphs_on_streams_and_with_non_finite_rows(m, dtype):
+    from chocosgd_b200.ops.ffn import gated_ffn
+
+    x, wi, wo, _ = _inputs(m, 650, 1300, 650, dtype)
+    want = gated_ffn(x, wi, wo)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+            with torch.cuda.stream(s):
+                outs.append(gated_ffn(x, wi, wo))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):                                 # two calls in a row, the second on the first one's result
+        y = gated_ffn(gated_ffn(x, wi, wo), wi, wo)
+    x.mul_(-1)
+    wo.mul_(2)
+    g.replay()
+    assert torch.equal(y, gated_ffn(gated_ffn(x, wi, wo), wi, wo))
+    clean = gated_ffn(x, wi, wo)
+    x[0, 7], x[m - 1] = float("nan"), float("inf")
+    y = gated_ffn(x, wi, wo)
+    assert torch.equal(y[1:m - 1], clean[1:m - 1]) and torch.isnan(y[0]).all() and not torch.isfinite(y[m - 1]).any()
+
+
+@pytest.mark.gpu
+def test_few_tokens_do_not_touch_what_lies_beside_the_result():
+    """Rows of a view whose neighbours are not finite: neither read into the sums nor written."""
+    from chocosgd_b200.ops.ffn import gated_ffn
+
+    for dtype in DTYPES:
+        for m in (3, 13, 29):
+            x, wi, wo, _ = _inputs(m, 70, 90, 50, dtype)
+            want = gated_ffn(x, wi, wo)
+            views = []
+            for t in (x, wi, wo):
+                wide = torch.full((t.size(0) + 2, t.size(1) + 10), float("nan"), dtype=dtype, device="cuda")
+                wide[1:-1, 2:-8] = t
+                views.append(wide[1:-1, 2:-8])
+            assert torch.equal(gated_ffn(*views), want)
+
+
+@pytest.mark.gpu
 def test_leading_dimensions_strides_and_broadcast_gradients():
     from chocosgd_b200.ops.ffn import gated_ffn
 
