@@ -56,6 +56,19 @@ Tensor rows_of(const Tensor& t) {
 }
 // elements from row to row (a single row's stride says nothing)
 long long pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max<long long>(1, t.size(1)); }
+// Saved tensors come back through hooks (offloading, recomputation), and a leaf's .data can be assigned to in between: the
+// values are the same, strides and alignment need not be.  Size, type and device have to.
+void check_saved(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& device, const char* what) {
+  if (t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device) return;
+  std::ostringstream s;
+  s << what << ": a saved tensor came back as " << describe(t) << ", it was " << sizes << " " << type << " " << device;
+  throw std::runtime_error(s.str());
+}
+// a workspace as the kernels need it: one run of bytes on a 256-byte boundary
+Tensor workspace_of(const Tensor& t) {
+  if (t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 256 == 0) return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
 Tensor empty(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, like.options()); }
 Tensor empty_floats(long long n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 
@@ -204,17 +217,26 @@ struct Layout {
     return at;
   }
   // room for the operand image of a matrix, or none where it is read as it is
+  static bool direct(const Tensor& t) {
+    return t.scalar_type() != at::kFloat && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && pitch(t) % 8 == 0;
+  }
   long long image(const Tensor& t) {
-    if (t.scalar_type() != at::kFloat && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && pitch(t) % 8 == 0) return -1;
+    if (direct(t)) return -1;
     return add(t.size(0) * pad(t.size(1), 16) * (t.scalar_type() == at::kFloat ? 6 : 2));
   }
 };
 void* at_offset(const Tensor& buf, long long offset) { return offset < 0 ? nullptr : static_cast<char*>(buf.data_ptr()) + offset; }
 
-// what the forward pass leaves: images of the three operands, the hidden values and (training) G and U
+// Byte offsets of what the forward pass leaves in its workspace: images of the three operands, the hidden values and (training) G and U.
+// The backward pass takes them from its node: which operands needed an image was decided by the tensors of the forward pass.
 struct FfnBuffers {
   Layout layout;
-  long long x, w_in, w_out, h, z;
+  long long x = -1, w_in = -1, w_out = -1, h = -1, z = -1;
+  FfnBuffers() = default;
+  explicit FfnBuffers(const std::vector<int64_t>& kept) : x(kept[0]), w_in(kept[1]), w_out(kept[2]), h(kept[3]), z(kept[4]) {
+    layout.size = kept[5];
+  }
+  std::vector<int64_t> keep() const { return {x, w_in, w_out, h, z, layout.size}; }
   FfnBuffers(const Tensor& x2, const Tensor& wi, const Tensor& wo, bool train, bool few) {
     const long long m = x2.size(0), f = pad(wo.size(1), 16), planes = x2.scalar_type() == at::kFloat ? 3 : 1;
     x = few ? -1 : layout.image(x2);
@@ -226,7 +248,8 @@ struct FfnBuffers {
 };
 Tensor bytes(long long n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
-Tensor ffn_run(const Tensor& x, const Tensor& x2, const Tensor& wi, const Tensor& wo, int64_t act, bool train, Tensor* kept) {
+Tensor ffn_run(const Tensor& x, const Tensor& x2, const Tensor& wi, const Tensor& wo, int64_t act, bool train, Tensor* kept,
+               FfnBuffers* at_kept) {
   const int m = (int)x2.size(0), d = (int)x2.size(1), f = (int)wo.size(1), n = (int)wo.size(0), dt = dtype_code(x.scalar_type());
   const bool few = !train && gated_ffn_few(m, d, f, n, dt);
   std::vector<int64_t> shape = x.sizes().vec();
@@ -240,6 +263,7 @@ Tensor ffn_run(const Tensor& x, const Tensor& x2, const Tensor& wi, const Tensor
   Tensor buf = bytes(at.layout.size, x);
   const long long floats = few ? 0 : gated_ffn_partial_floats(m, d, f, n, dt, 0);
   if (floats) partial = empty_floats(floats, x);
+  *at_kept = at;
   FfnForwardCall c = {};
   c.x = x2.data_ptr(); c.ldx = pitch(x2); c.x_img = at_offset(buf, at.x);
   c.w_in = wi.data_ptr(); c.ld_in = pitch(wi); c.in_img = at_offset(buf, at.w_in);
@@ -259,38 +283,51 @@ Tensor ffn_run(const Tensor& x, const Tensor& x2, const Tensor& wi, const Tensor
 struct GatedFfnFn : torch::autograd::Function<GatedFfnFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act) {
     const Tensor x2 = rows_of(x), wi = rows_of(w_in), wo = rows_of(w_out);
-    Tensor buf, y = ffn_run(x, x2, wi, wo, act, true, &buf);
+    Tensor buf;
+    FfnBuffers at;
+    Tensor y = ffn_run(x, x2, wi, wo, act, true, &buf, &at);
     ctx->save_for_backward({x2, wi, wo, buf});
     ctx->saved_data["act"] = act;
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x2.size(0), x2.size(1), wo.size(1), wo.size(0)};
+    ctx->saved_data["buffers"] = at.keep();
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("gated_ffn");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x2 = saved[0], &wi = saved[1], &wo = saved[2], &buf = saved[3], &dy = grads[0];
-    const int m = (int)x2.size(0), d = (int)x2.size(1), f = (int)wo.size(1), n = (int)wo.size(0), dt = dtype_code(x2.scalar_type());
-    const c10::OptionalDeviceGuard guard(x2.device());
+    const Tensor& dy = grads[0];
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const FfnBuffers at(ctx->saved_data["buffers"].toIntVector());
+    const int m = (int)sizes[0], d = (int)sizes[1], f = (int)sizes[2], n = (int)sizes[3], dt = dtype_code(dy.scalar_type());
+    check_saved(saved[0], {m, d}, dy.scalar_type(), dy.device(), "gated_ffn");
+    check_saved(saved[1], {2 * f, d}, dy.scalar_type(), dy.device(), "gated_ffn");
+    check_saved(saved[2], {n, f}, dy.scalar_type(), dy.device(), "gated_ffn");
+    check_saved(saved[3], {at.layout.size}, at::kByte, dy.device(), "gated_ffn");
+    const c10::OptionalDeviceGuard guard(dy.device());
     std::vector<int64_t> shape = dy.sizes().vec();
     shape.back() = d;
     Tensor dx, dwi, dwo;
-    if (ctx->needs_input_grad(0)) dx = empty(shape, x2);
-    if (ctx->needs_input_grad(1)) dwi = empty({2 * f, d}, x2);
-    if (ctx->needs_input_grad(2)) dwo = empty({n, f}, x2);
+    if (ctx->needs_input_grad(0)) dx = empty(shape, dy);
+    if (ctx->needs_input_grad(1)) dwi = empty({2 * f, d}, dy);
+    if (ctx->needs_input_grad(2)) dwo = empty({n, f}, dy);
     if (m == 0) {
       if (dwi.defined()) dwi.zero_();
       if (dwo.defined()) dwo.zero_();
       return {dx, dwi, dwo, Tensor()};
     }
-    const FfnBuffers at(x2, wi, wo, true, false);
-    const Tensor dy2 = rows_of(dy);
+    const Tensor x2 = rows_of(saved[0]), wi = rows_of(saved[1]), wo = rows_of(saved[2]), buf = workspace_of(saved[3]), dy2 = rows_of(dy);
     Layout scratch;
-    const long long dy_img = scratch.image(dy2), dz = scratch.add((dt == 0 ? 3 : 1) * 4LL * m * pad(f, 16));
+    // operands that the forward pass read as they were and that came back otherwise get an image now
+    const long long dy_img = scratch.image(dy2), x_img = at.x < 0 ? scratch.image(x2) : -1, in_img = at.w_in < 0 ? scratch.image(wi) : -1,
+                    out_img = at.w_out < 0 ? scratch.image(wo) : -1;
+    const long long dz = scratch.add((dt == 0 ? 3 : 1) * 4LL * m * pad(f, 16));
     const long long floats = gated_ffn_partial_floats(m, d, f, n, dt, 1), partial = floats ? scratch.add(4 * floats) : -1;
-    const Tensor s = bytes(scratch.size, x2);
+    const Tensor s = bytes(scratch.size, dy);
     FfnBackwardCall c = {};
-    c.x = x2.data_ptr(); c.ldx = pitch(x2); c.x_img = at_offset(buf, at.x);
-    c.w_in = wi.data_ptr(); c.ld_in = pitch(wi); c.in_img = at_offset(buf, at.w_in);
-    c.w_out = wo.data_ptr(); c.ld_out = pitch(wo); c.out_img = at_offset(buf, at.w_out);
+    c.x = x2.data_ptr(); c.ldx = pitch(x2); c.x_img = x_img >= 0 ? at_offset(s, x_img) : at_offset(buf, at.x);
+    c.w_in = wi.data_ptr(); c.ld_in = pitch(wi); c.in_img = in_img >= 0 ? at_offset(s, in_img) : at_offset(buf, at.w_in);
+    c.w_out = wo.data_ptr(); c.ld_out = pitch(wo); c.out_img = out_img >= 0 ? at_offset(s, out_img) : at_offset(buf, at.w_out);
+    c.make = (x_img >= 0 ? 1 : 0) | (in_img >= 0 ? 2 : 0) | (out_img >= 0 ? 4 : 0);
     c.dy = dy2.data_ptr(); c.ldy = pitch(dy2); c.dy_img = at_offset(s, dy_img);
     c.h = at_offset(buf, at.h);
     c.z = static_cast<float*>(at_offset(buf, at.z));
@@ -298,9 +335,9 @@ struct GatedFfnFn : torch::autograd::Function<GatedFfnFn> {
     c.partial = static_cast<float*>(at_offset(s, partial));
     c.dx = ptr(dx); c.dw_in = ptr(dwi); c.dw_out = ptr(dwo);
     c.m = m; c.d = d; c.f = f; c.n = n; c.act = ctx->saved_data["act"].toInt(); c.dt = dt;
-    c.st = stream_of(x2);
+    c.st = stream_of(dy);
     check(gated_ffn_backward(&c), "gated_ffn_backward");
-    g_launches += 1 + (dx.defined() || dwi.defined()) + (dy_img >= 0) + (floats > 0);
+    g_launches += 1 + (dx.defined() || dwi.defined()) + (dy_img >= 0 || c.make != 0) + (floats > 0);
     return {dx, dwi, dwo, Tensor()};
   }
 };
@@ -325,7 +362,8 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w_in) || wants_grad(w_out)))
     return GatedFfnFn::apply(x, w_in, w_out, act);
   Tensor buf;
-  return ffn_run(x, rows_of(x), rows_of(w_in), rows_of(w_out), act, false, &buf);
+  FfnBuffers at;
+  return ffn_run(x, rows_of(x), rows_of(w_in), rows_of(w_out), act, false, &buf, &at);
 }
 
 }  // namespace

@@ -58,7 +58,8 @@ struct FfnForwardCall {
   void* st;
 };
 
-// x, w_in, w_out: as in the forward pass; where an image is given it holds the forward pass' image already.
+// x, w_in, w_out: as in the forward pass; where an image is given it holds the forward pass' image already, or (bits 0, 1, 2 of
+// `make`) is scratch for one that is still to be made.
 // dz: [S][2][m][pad16(f)] 16-bit scratch.  dx, dw_in, dw_out may be null.
 struct FfnBackwardCall {
   const void* x;
@@ -78,7 +79,7 @@ struct FfnBackwardCall {
   void* dz;
   float* partial;
   void *dx, *dw_in, *dw_out;
-  long long m, d, f, n, act, dt;
+  long long make, m, d, f, n, act, dt;
   void* st;
 };
 

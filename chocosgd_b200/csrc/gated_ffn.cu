@@ -693,7 +693,7 @@ struct FfnImage {
   unsigned first_block;     // blocks [first_block, next image's) copy this matrix, eight elements per thread
 };
 struct FfnImages {
-  FfnImage m[3];
+  FfnImage m[4];
   int n;
 };
 template <int S>
@@ -1115,9 +1115,9 @@ extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
   FfnOperand ox, oi, oo, oy;
   FfnImages images = {};
   ffn_prepare(&oy, dy, m, n, ldy, 1, dt, dy_img, &images);
-  ffn_prepare(&ox, x_img != nullptr ? nullptr : x, m, d, ldx, 1, dt, x_img, &images);
-  ffn_prepare(&oi, in_img != nullptr ? nullptr : w_in, 2LL * f, d, ld_in, 2, dt, in_img, &images);
-  ffn_prepare(&oo, out_img != nullptr ? nullptr : w_out, n, f, ld_out, 1, dt, out_img, &images);
+  ffn_prepare(&ox, x_img != nullptr && !(c->make & 1) ? nullptr : x, m, d, ldx, 1, dt, x_img, &images);
+  ffn_prepare(&oi, in_img != nullptr && !(c->make & 2) ? nullptr : w_in, 2LL * f, d, ld_in, 2, dt, in_img, &images);
+  ffn_prepare(&oo, out_img != nullptr && !(c->make & 4) ? nullptr : w_out, n, f, ld_out, 1, dt, out_img, &images);
   int rc = ffn_make_images(images, dt, st);
   if (rc) return rc;
   const FfnOperand oh = {h, m, f, 1, S, pad16(f)}, oz = {dz, m, f, 2, S, pad16(f)};
