@@ -110,14 +110,20 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const Tensor x2 = rows_of(x), stats = empty_floats(2 * x2.size(0), x);
     ctx->save_for_backward({x2, w, stats});
     ctx->saved_data["type"] = static_cast<int64_t>((w.defined() ? w : (b.defined() ? b : x)).scalar_type());
+    ctx->saved_data["rows"] = x2.size(0);
     return layer_norm_run(x, x2, w, b, eps, stats);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("layer_norm");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x2 = saved[0], &w = saved[1], &stats = saved[2], dy2 = rows_of(grads[0]);
+    const Tensor dy2 = rows_of(grads[0]);
+    const int64_t rows = ctx->saved_data["rows"].toInt(), width = dy2.size(1);
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
-    const c10::OptionalDeviceGuard guard(x2.device());
+    check_saved(saved[0], {rows, width}, dy2.scalar_type(), dy2.device(), "layer_norm");
+    if (saved[1].defined()) check_saved(saved[1], {width}, type, dy2.device(), "layer_norm");
+    check_saved(saved[2], {2 * rows}, at::kFloat, dy2.device(), "layer_norm");
+    const c10::OptionalDeviceGuard guard(dy2.device());
+    const Tensor x2 = rows_of(saved[0]), w = saved[1].defined() ? saved[1].contiguous() : saved[1], stats = saved[2].contiguous();
     Tensor dx, dw, db, partial;
     if (ctx->needs_input_grad(0)) dx = empty(grads[0].sizes(), x2);
     const size_t bias_index = w.defined() ? 2 : 1;
@@ -181,6 +187,8 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor key = ctx->get_saved_variables()[0], &dy = grads[0];
+    static const int64_t one = 1;
+    check_saved(key, key.numel() == 1 ? key.sizes() : at::IntArrayRef(one), at::kLong, dy.device(), "dropout");
     const int64_t drop = ctx->saved_data["drop"].toInt(), site = ctx->saved_data["site"].toInt();
     const c10::OptionalDeviceGuard guard(dy.device());
     Tensor dx, dr;

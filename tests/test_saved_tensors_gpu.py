@@ -3,6 +3,8 @@ with other strides and another alignment give the same bits, another size, type 
 import pytest
 import torch
 
+from test_norm_gpu import U, _plain
+
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
@@ -144,3 +146,69 @@ def test_gated_ffn_in_a_checkpoint(dtype):
         y.backward(dy)
         for t, b in zip(leaves, want):
             assert torch.equal(t.grad, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,w_dtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("view", sorted(VIEWS))
+@pytest.mark.parametrize("shape", [(41, 131), (300, 256), (2, 3, 65), (3, 16385)])
+def test_layer_norm(shape, view, dtype, w_dtype):
+    from chocosgd_b200.ops.norm import layer_norm
+
+    g = torch.Generator(device="cuda").manual_seed(sum(shape))
+    x = VIEWS[view](torch.randn(*shape, device="cuda", generator=g).to(dtype)).requires_grad_()
+    w = VIEWS["off"](torch.randn(shape[-1], device="cuda", generator=g).to(w_dtype)).requires_grad_()
+    b = torch.randn(shape[-1], device="cuda", generator=g).to(w_dtype).requires_grad_()
+    dy = torch.randn(*shape, device="cuda", generator=g).to(dtype)
+    want = torch.autograd.grad(layer_norm(x, w, b), (x, w, b), dy)
+    # Another alignment may take the kernel of another access width, which adds up in another order.  Twice the bound of either side
+    # against 64 bits: z within zerr, the two means within 32 roundings of their terms, sums over rows of at most depth additions.
+    rdx, rdw, rdb, z, rs, gw, zerr = _plain(x.detach(), w, b, 1e-5, dy)[1:8]
+    dyd, lead = dy.double().abs(), tuple(range(len(shape) - 1))
+    u, uw, depth = U[dtype], U[w_dtype], 162
+    gm, gz = gw.abs().mean(-1, keepdim=True), (gw * z).abs().mean(-1, keepdim=True)
+    tol = (rs * (32 * 2.0 ** -24 * (gw.abs() + gm + z.abs() * gz) + zerr * gz + z.abs() * (gw.abs() * zerr).mean(-1, keepdim=True))
+           + u * rdx.abs() + 1e-7,
+           depth * 2.0 ** -24 * (dyd * z.abs()).sum(lead) + (dyd * zerr).sum(lead) + uw * rdw.abs() + 1e-7,
+           depth * 2.0 ** -24 * dyd.sum(lead) + uw * rdb.abs() + 1e-7)
+    for name in ("cpu", *sorted(UNPACK)):
+        with _hooks(name):
+            y = layer_norm(x, w, b)
+        for p, q, t in zip(torch.autograd.grad(y, (x, w, b), dy), want, tol):
+            assert ((p.double() - q.double()).abs() <= 2 * t).all(), name
+
+
+@pytest.mark.gpu
+def test_layer_norm_and_dropout_refuse_other_sizes_types_and_devices():
+    from chocosgd_b200.ops.dropout import dropout
+    from chocosgd_b200.ops.norm import layer_norm
+
+    w = torch.ones(64, device="cuda")
+    key = torch.tensor([3], device="cuda")
+    for call, saved in ((lambda x: layer_norm(x, w), 3), (lambda x: dropout(x, 0.5, key), 1)):
+        for which in range(saved):
+            for change in (lambda t: t[:-1], lambda t: t.repeat_interleave(2, 0), lambda t: t.cpu(), lambda t: t.to(torch.float64)):
+                x = torch.randn(30, 64, device="cuda").requires_grad_()
+                count = [0]
+
+                def unpack(t):
+                    count[0] += 1
+                    return change(t) if count[0] == which + 1 else t
+
+                with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                    y = call(x)
+                with pytest.raises(RuntimeError, match="saved tensor came back"):
+                    torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@pytest.mark.gpu
+def test_dropout():
+    from chocosgd_b200.ops.dropout import dropout
+
+    key = torch.tensor([41], device="cuda")
+    x, dy = torch.randn(1003, device="cuda").requires_grad_(), torch.randn(1003, device="cuda")
+    want = torch.autograd.grad(dropout(x, 0.4, key), x, dy)[0]
+    for name in ("cpu", *sorted(UNPACK)):
+        with _hooks(name):
+            y = dropout(x, 0.4, key)
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], want), name
