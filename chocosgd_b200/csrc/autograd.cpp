@@ -44,6 +44,12 @@ std::string describe(const Tensor& t) {
   return s.str();
 }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// a tangent of forward-mode differentiation: the kernels would drop it without a word
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+void no_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), what, ": no forward-mode derivative (an input carries a tangent)");
+}
 void no_second_derivative(const char* what) {
   if (at::GradMode::is_enabled())
     throw std::runtime_error(std::string(what) + ": the backward kernels have no derivative (create_graph=True)");
@@ -155,6 +161,7 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, doubl
     throw pybind11::value_error(
         "layer_norm: needs a CUDA tensor of fp32, bf16 or fp16 and, where given, weight and bias of its last dimension's length on "
         "its device, both of its type or both fp32: got " + describe(x) + ", " + describe(w) + ", " + describe(b));
+  no_tangent("layer_norm", {&x, &w, &b});
   const c10::OptionalDeviceGuard guard(x.device());
   if (w.defined()) w = w.contiguous();
   if (b.defined()) b = b.contiguous();
@@ -208,6 +215,7 @@ Tensor dropout(const Tensor& x, int64_t drop, const Tensor& key, int64_t site, c
     throw pybind11::value_error("dropout: the key is one 64-bit integer on the input's device (new_key), got " + describe(key));
   if (residual.defined() && !(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type() && residual.device() == x.device()))
     throw pybind11::value_error("dropout: the residual has the input's shape, type and device, got " + describe(residual) + " for " + describe(x));
+  no_tangent("dropout", {&x, &residual});
   const c10::OptionalDeviceGuard guard(x.device());
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(residual))) return DropoutFn::apply(x, maybe(residual), key, drop, site);
   return dropout_run(x, residual, key, drop, site);
@@ -366,6 +374,7 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64
     throw pybind11::value_error(
         "gated_ffn: needs x [..., D], w_in [2 F, D] and w_out [N, F] on one CUDA device and of one type (fp32, bf16 or fp16): got " +
         describe(x) + ", " + describe(w_in) + ", " + describe(w_out));
+  no_tangent("gated_ffn", {&x, &w_in, &w_out});
   const c10::OptionalDeviceGuard guard(x.device());
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w_in) || wants_grad(w_out)))
     return GatedFfnFn::apply(x, w_in, w_out, act);
@@ -379,11 +388,15 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // wrapped: an allocation that fails raises PyTorch's own exception
   m.def("layer_norm", torch::wrap_pybind_function(layer_norm));
-  m.def("layer_norm_supported", [](const Tensor& x, const Maybe& w, const Maybe& b) {
-    return layer_norm_ok(x, w.value_or(Tensor()), b.value_or(Tensor()));
+  m.def("layer_norm_supported", [](const Tensor& x, const Maybe& weight, const Maybe& bias) {
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    return layer_norm_ok(x, w, b) && !has_tangent(x) && !has_tangent(w) && !has_tangent(b);
   });
   m.def("dropout", torch::wrap_pybind_function(dropout));
   m.def("gated_ffn", torch::wrap_pybind_function(gated_ffn));
-  m.def("gated_ffn_supported", &gated_ffn_ok);
+  m.def("gated_ffn_supported", [](const Tensor& x, const Tensor& w_in, const Tensor& w_out) {
+    return gated_ffn_ok(x, w_in, w_out) && !has_tangent(x) && !has_tangent(w_in) && !has_tangent(w_out);
+  });
+  m.def("has_tangent", &has_tangent);
   m.def("launches", []() { return g_launches.load(); });
 }

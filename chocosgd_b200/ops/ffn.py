@@ -7,7 +7,8 @@ one type.  16-bit operands are multiplied as they are with fp32 accumulators, th
 fp32 operands are split into three bf16 parts each and keep fp32 accuracy (a row that holds an infinity gives
 non-finite results, not always the infinity itself; so does a hidden value above fp16's range with fp16 operands).  Rows that do not start on 16-byte boundaries (and
 fp32 operands) are re-laid into an image of the operand first; the backward pass uses the forward pass' images.  Without a gradient
-and for few tokens (up to 4, fp32: 32) the weights are read once as they are, without tensor cores."""
+and for few tokens (up to 4, fp32: 32) the weights are read once as they are, without tensor cores.  Neither the backward pass' own derivative nor a forward-mode one exists;
+both are refused."""
 from __future__ import annotations
 
 from . import _lib

@@ -161,7 +161,7 @@ class Dropout(nn.Dropout):
         if on and self.training and self.p > 0 and not self.inplace and x.is_cuda:
             from .dropout import dropout, dropout_supported, new_key
 
-            if dropout_supported(x):
+            if dropout_supported(x, residual):
                 if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
                     return residual + dropout(x, self.p, new_key(x.device))
                 return dropout(x, self.p, new_key(x.device), residual=residual)

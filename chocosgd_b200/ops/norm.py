@@ -4,7 +4,8 @@ checks of the arguments: ``csrc/autograd.cpp``).
 ``layer_norm(x, weight, bias, eps)`` is ``torch.nn.functional.layer_norm`` for one normalised dimension: ``x`` fp32, bf16
 or fp16 of any leading shape (rows may be strided, the last dimension has to be contiguous), ``weight`` / ``bias`` of ``x``'s
 type or fp32, either of them may be ``None``.  Statistics and sums are fp32.  The parameters' gradients are summed in a fixed
-order: the same inputs give the same bits.  The backward pass has no derivative of its own and says so."""
+order: the same inputs give the same bits.  The backward pass has no derivative of its own and says so; there is
+no forward-mode derivative, a dual tensor is refused (the layer class takes the library's path for it)."""
 from __future__ import annotations
 
 from . import _lib
