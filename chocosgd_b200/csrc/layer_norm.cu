@@ -25,9 +25,14 @@
 #include "tc_common.cuh"
 #include "vec.cuh"
 
+#include <atomic>
+
 #define LN_MAX_ROW 16384
 
-__device__ int g_ln_error;      // a bounded wait ran out
+// A wait of the rings is bounded.  A warp whose wait runs out sets the error word and goes on in ln_fwd_late or ln_bwd_late: it waits
+// no more, meets its group's barriers with NaN for its share of the sums, so that the group's remaining rows become NaN as a whole, and its
+// columns of dw and db are NaN.  The thread that starts the copies also waits for those in flight and starts none again.
+__device__ int g_ln_error;
 
 struct LnArgs {
   const void* x;        // [N, D], ldx elements per row
@@ -118,6 +123,47 @@ __device__ __forceinline__ void ln_bulk(void* dst, const void* src, uint32_t byt
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+#define LN_NAN __int_as_float(0x7FC00000)
+// where a group stands: its row, the stage k of that row and the parity of its barrier; depth stages, copies of `ahead` rows under way
+struct LnRing {
+  uint64_t* full;
+  int k, depth, ahead;
+  uint32_t phase;
+  long long row, stride, n;
+};
+__device__ __forceinline__ void ln_gave_up(const LnRing& r, int t) {
+  atomicExch(&g_ln_error, 1);
+  if (t != 0) return;
+  for (int j = 0; j < r.ahead && r.row + j * r.stride < r.n; ++j)
+    mbar_wait(r.full + (r.k + j) % r.depth, r.phase ^ (r.k + j >= r.depth ? 1u : 0u));
+}
+template <typename T>
+__device__ __forceinline__ void ln_nan_row(T* row, int d, int t, int threads) {
+  constexpr int V = 16 / sizeof(T);
+  for (int v = t; v < d / V; v += threads)
+    for (int e = 0; e < V; ++e) row[v * V + e] = from_f<T>(LN_NAN);
+}
+template <typename T>
+__device__ __noinline__ void ln_fwd_late(LnRing r, float* red, T* y, float* mean, float* rstd, int d, int group, int t, int threads) {
+  ln_gave_up(r, t);
+  for (long long row = r.row; row < r.n; row += r.stride) {
+    float s[1] = {LN_NAN};
+    ln_group_sum<1>(s, red, group, t, threads);
+    ln_group_sum<1>(s, red + 32, group, t, threads);
+    ln_nan_row(y + row * d, d, t, threads);
+    if (t == 0 && mean != nullptr) mean[row] = rstd[row] = LN_NAN;
+  }
+}
+template <typename T>
+__device__ __noinline__ void ln_bwd_late(LnRing r, int turn, float* red, T* dx, int d, int group, int t, int threads) {
+  ln_gave_up(r, t);
+  for (long long row = r.row; row < r.n; row += r.stride, turn ^= 1) {
+    float s[2] = {LN_NAN, LN_NAN};
+    ln_group_sum<2>(s, red + turn * 64, group, t, threads);
+    if (dx != nullptr) ln_nan_row(dx + row * d, d, t, threads);
+  }
+}
+
 // parameters of vector v as pairs
 template <int V>
 __device__ __forceinline__ void ln_get2(const float* s, int vectors, int v, F2 (&out)[V / 2]) {
@@ -134,7 +180,8 @@ __device__ __forceinline__ void ln_get2(const float* s, int vectors, int v, F2 (
 // the registers have it.  Arithmetic in pairs of fp32 numbers: one element at a time the kernel is bound by issue (18 instructions
 // per element; 16384 x 4096 bf16: 85 us, with pairs and 8 vectors per lane 77, with 4 vectors 63,
 // with 768 threads 57; 65536 x 1024: 48).
-template <typename T, int NV>
+// GIVE_UP: the first wait counts as one that ran out (tests).
+template <typename T, int NV, bool GIVE_UP>
 __global__ void __launch_bounds__(768, 1) ln_fwd_ring_kernel(LnArgs a, int threads, int groups, int depth) {
   constexpr int V = 16 / sizeof(T);
   extern __shared__ float4 ln_smem4[];
@@ -168,7 +215,11 @@ __global__ void __launch_bounds__(768, 1) ln_fwd_ring_kernel(LnArgs a, int threa
   int k = 0;
   uint32_t phase = 0;
   for (long long row = first; row < a.n; row += stride) {
-    if (!mbar_wait(&full[group][k], phase)) atomicExch(&g_ln_error, 1);
+    if (GIVE_UP || !__all_sync(0xffffffffu, mbar_wait(&full[group][k], phase))) {
+      ln_fwd_late({full[group], k, depth, depth, phase, row, stride, a.n}, red[group][0], reinterpret_cast<T*>(a.y), a.mean, a.rstd, a.d,
+                  group, t, threads);
+      break;
+    }
     Vec<T, V> r[NV];
     F2 sum = f2(0.f), more = f2(0.f);
 #pragma unroll
@@ -297,7 +348,7 @@ __global__ void __launch_bounds__(256, NV >= 16 ? 2 : 4) ln_fwd_kernel(LnArgs a,
 // Rows on 16-byte boundaries.  x and dy of a row lie in a stage of the group's ring and are read there twice, before and after
 // the row's two sums are known; registers hold only the sums of dw and db.  The stage
 // of the row before is filled again behind the barrier of the row's sums: by then every thread is done with it.
-template <typename T, int E>
+template <typename T, int E, bool GIVE_UP>
 __global__ void __launch_bounds__(E == 8 ? 1024 : LN_T16, 1) ln_bwd_ring_kernel(LnArgs a, int threads, int groups) {
   constexpr int V = 16 / sizeof(T), NV = E / V;
   extern __shared__ float4 ln_smem4[];
@@ -339,7 +390,13 @@ __global__ void __launch_bounds__(E == 8 ? 1024 : LN_T16, 1) ln_bwd_ring_kernel(
       next_mu = a.mean[row + stride];
       next_rs = a.rstd[row + stride];
     }
-    if (!mbar_wait(&full[group][k], phase)) atomicExch(&g_ln_error, 1);
+    if (GIVE_UP || !__all_sync(0xffffffffu, mbar_wait(&full[group][k], phase))) {
+      ln_bwd_late({full[group], k, LN_RING, LN_RING - 1, phase, row, stride, a.n}, turn, red[group][0], reinterpret_cast<T*>(a.dx), a.d,
+                  group, t, threads);
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) dw[e] = db[e] = f2(LN_NAN);
+      break;
+    }
     const uint4 *xs = reinterpret_cast<const uint4*>(mine + k * 2 * row_bytes), *gs = xs + vectors;
     const F2 rs2 = f2(rs), off = f2(-mu * rs);
     F2 s0 = f2(0.f), s1 = f2(0.f);
@@ -584,6 +641,10 @@ __global__ void __launch_bounds__(256) ln_wgrad_long_kernel(LnArgs a) {
 }
 
 // ---------------------------------- host side ----------------------------------------------
+static std::atomic<int> ln_give_up{0};
+// 1: in the launches that follow every row group takes its first wait for one that ran out (for tests of what happens then); returns the state before
+extern "C" int layer_norm_give_up(int on) { return ln_give_up.exchange(on); }
+
 // elements per access: as many as the common alignment of all row starts allows
 static int ln_vec(const LnArgs& a, int dt, bool bwd) {
   const int es = dt_bytes(dt);
@@ -630,7 +691,7 @@ static int ln_launch_fwd_ring(const LnArgs& a, cudaStream_t st, bool* done) {
   if ((long long)groups * depth * row_bytes > 96 * 1024 && depth > 3) depth = 3;      // about what covers the latency
   *done = true;
   const int smem = 8 * a.d + groups * depth * row_bytes;
-  void (*kernel)(LnArgs, int, int, int) = ln_fwd_ring_kernel<T, NV>;
+  void (*kernel)(LnArgs, int, int, int) = ln_give_up ? ln_fwd_ring_kernel<T, NV, true> : ln_fwd_ring_kernel<T, NV, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
   const long long blocks = (a.n + groups - 1) / groups, most = sm_count();
@@ -679,7 +740,7 @@ static int ln_launch_bwd(const LnArgs& a, int* blocks, cudaStream_t st) {
   if (nb > sm_count()) nb = sm_count();
   *blocks = (int)nb;
   void (*kernel)(LnArgs, int, int) = nullptr;
-  if constexpr (RING) kernel = ln_bwd_ring_kernel<T, E>;
+  if constexpr (RING) kernel = ln_give_up ? ln_bwd_ring_kernel<T, E, true> : ln_bwd_ring_kernel<T, E, false>;
   else kernel = ln_bwd_kernel<T, V, E>;
   if (smem > 16 * 1024) {      // set for every launch: the attribute belongs to the current device
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -756,9 +817,11 @@ extern "C" int layer_norm_backward(const LnBackwardCall* c) {
                        (const float*)c->partial, blocks, a.d, c->dw, c->db, a.w_dt);
 }
 
-// 0, or 1 after a bounded wait of the backward kernel on the current device ran out (synchronises)
+// 0, or 1 after a bounded wait of a kernel on the current device ran out since the last call (synchronises)
 extern "C" int layer_norm_last_error() {
   int v = -1;
-  cudaMemcpyFromSymbol(&v, g_ln_error, sizeof(int));
+  if (cudaMemcpyFromSymbol(&v, g_ln_error, sizeof(int)) != cudaSuccess) return -1;
+  const int none = 0;
+  if (v != 0) cudaMemcpyToSymbol(g_ln_error, &none, sizeof(int));
   return v;
 }
