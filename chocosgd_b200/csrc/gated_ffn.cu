@@ -32,11 +32,14 @@
 // 178, 175 and 882 us without activation, G, U or their gradients.  fp32, 1120 x 650 x 2600: gate 52 us, Y 33 + 6, dgate 48, the
 // gradients 125 + 8, images 16; there the epilogue, which takes the accumulator out every 32 k, costs as much as the products.
 //
-// Every mbarrier wait is bounded; a wait that runs out sets the error word, the CTA drains and frees its TMEM.
+// Every mbarrier wait is bounded.  A wait that runs out ends the work of its CTA (both CTAs of a pair): results that are not written by
+// then stay unwritten, the copies and multiplications in flight are waited for, TMEM is freed and the error word is set.
 #include "block_calls.h"
 #include "launch.cuh"
 #include "tc_common.cuh"
 #include "ffn.cuh"
+
+#include <atomic>
 
 #define FF_BM 128            // accumulator rows of one CTA
 #define FF_BK(S) ((S) == 3 ? 32 : 64)    // k per stage: K-major rows of 64 (three planes) or 128 bytes = one swizzle row
@@ -72,6 +75,7 @@ struct FfnGemm {
 struct FfnBatch {
   FfnGemm g[3];
   int n, first[4];
+  int give_up;           // not 0 (tests): CTAs of the ranks in bits 0 and 1 act after (give_up >> 2) ns as if a wait had run out
 };
 
 // fp32 matrices that only these kernels read (G, U, partial sums) are stored in the order in which a warp of the epilogue
@@ -177,6 +181,31 @@ __device__ __forceinline__ void tmem_wait16(float* v) {
                : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
                  "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
+// as mbar_wait, and false too once the CTA (or its peer) has given up
+__device__ __forceinline__ bool ff_wait(uint64_t* bar, uint32_t parity, const volatile int* abort_flag) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+    if (ok) return true;
+    if (i > 1024) {
+      if (*abort_flag != 0) return false;
+      __nanosleep(64);
+    }
+  }
+  return false;
+}
+// ends the work of this CTA, and of its peer
+template <int CG>
+__device__ __forceinline__ void ff_give_up(volatile int* abort_flag, uint32_t rank) {
+  *abort_flag = 1;
+  if (CG == 2)
+    asm volatile("st.volatile.shared::cluster.u32 [%0], %1;" ::"r"(map_rank(const_cast<const int*>(abort_flag), rank ^ 1)), "r"(1) : "memory");
+}
 template <int EPI>
 __device__ __forceinline__ bool ff_epi_bar_or(bool flag) {
   uint32_t r;
@@ -187,6 +216,16 @@ __device__ __forceinline__ bool ff_epi_bar_or(bool flag) {
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(r) : "r"((uint32_t)flag), "n"(EPI * 32) : "memory");
   return r != 0;
+}
+
+// a word of the peer's shared memory
+__device__ __forceinline__ uint32_t ff_peer_word(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.volatile.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void ff_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // 32 bytes of a row with one access: a whole sector, although the lanes of a warp are in different rows
@@ -364,6 +403,7 @@ template <int BN, int S, int KIND, int CG> struct FfnSmem {
   static constexpr int EPI_BYTES = EPI * 4096;            // 4 KB for each epilogue warp
   static constexpr int ROOM = 227 * 1024 - 256 - 1024 - EPI_BYTES;
   static constexpr int STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
+  static_assert((2 * STAGES + 5) * 8 + 12 <= 256, "barriers and words");
   static constexpr int BYTES = STAGES * STAGE + EPI_BYTES + 256 + 1024;
 };
 
@@ -424,8 +464,10 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
   uint64_t* empty = full + L::STAGES;
   uint64_t* acc_full = empty + L::STAGES;    // [2]
   uint64_t* acc_empty = acc_full + 2;        // [2], the leader's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* drained = acc_empty + 2;         // after a wait that ran out
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* issued = tmem_slot + 2; // stages that this CTA's copies were started for
   constexpr int BN_OUT = KIND == FF_GATE ? BN / 2 : BN;    // output columns of a tile
   constexpr int TM = FF_BM * CG;                           // output rows of a tile
 
@@ -444,6 +486,7 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
       mbar_init(acc_full + b, 1);
       mbar_init(acc_empty + b, L::EPI * CG);   // one arrival per epilogue warp
     }
+    mbar_init(drained, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -471,7 +514,7 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
         for (int i = at.kb0; i < at.kb1; ++i) {
           const int seg = i >= g.k_blocks ? 1 : 0, k0 = (i - seg * g.k_blocks) * BK;
           const int part_a = g.m_parts > 1 ? m_part : (g.a_parts > 1 ? seg : 0), part_b = g.b_parts > 1 ? seg : 0;
-          ok = __all_sync(0xffffffffu, mbar_wait(empty + s, phase) && *abort_flag == 0);
+          ok = __all_sync(0xffffffffu, ff_wait(empty + s, phase, abort_flag) && *abort_flag == 0);
           if (!ok) break;
           if (elect_one()) {
             if (rank == 0) mbar_expect_tx(full + s, CG * L::STAGE);
@@ -513,12 +556,8 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
         }
       }
     }
-    // after a wait that ran out: the copies in flight end before this CTA's shared memory is given back
-    if (!ok) {
-      *abort_flag = 1;
-      if (rank == 0)
-        for (uint32_t j = it > L::STAGES ? it - L::STAGES : 0; j < it; ++j) mbar_wait(full + j % L::STAGES, (j / L::STAGES) & 1);
-    }
+    if (lane == 0) *issued = it;
+    if (!ok) ff_give_up<CG>(abort_flag, rank);
   } else if (warp == L::EPI + 1 && rank == 0) {
     // ---------------- MMA issuer (of a pair: the leader's) ----------------
     uint32_t s = 0, phase = 0, chunk = 0;
@@ -542,8 +581,8 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
         const uint32_t buf = chunk & 1;
         const bool first = S == 3 || i == 0, last = S == 3 || i == n_kb - 1;      // S = 3: every k-block has its accumulator
         // the first round of either accumulator passes at once
-        if (first) ok = mbar_wait(acc_empty + buf, ((chunk >> 1) & 1) ^ 1);
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(full + s, phase));
+        if (first) ok = ff_wait(acc_empty + buf, ((chunk >> 1) & 1) ^ 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok && ff_wait(full + s, phase, abort_flag));
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -570,13 +609,17 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
         if (++s == L::STAGES) { s = 0; phase ^= 1; }
       }
     }
-    if (!ok) *abort_flag = 1;
+    if (!ok) ff_give_up<CG>(abort_flag, rank);
   } else if (warp < L::EPI) {
     // ---------------- epilogue: warp w reads lanes 32 (w % 4) ... of its share of the tile's output columns ----------------
     constexpr int HC = BN_OUT / (L::EPI / 4);         // output columns per warp
     const int half = warp >> 2;
     uint32_t chunk = 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    if (batch.give_up != 0 && threadIdx.x == 0 && (batch.give_up >> rank & 1)) {
+      __nanosleep((uint32_t)batch.give_up >> 2);
+      ff_give_up<CG>(abort_flag, rank);
+    }
     for (int tile = first_tile; tile < n_tiles; tile += tile_step) {
       const Where at(batch, tile, Where::which(batch, tile));
       const FfnGemm& g = at.g;
@@ -595,7 +638,7 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
         for (int c = 0; c < NA; ++c) acc[c] = 0.f;
         for (int i = at.kb0; i < at.kb1; ++i, ++chunk) {
           const uint32_t buf = chunk & 1;
-          const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
+          const bool bad = !ff_wait(acc_full + buf, (chunk >> 1) & 1, abort_flag) || *abort_flag != 0;
           if (ff_epi_bar_or<L::EPI>(bad)) { stop = true; break; }
           tc_fence_after();
 #pragma unroll
@@ -635,7 +678,7 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
         // while the tile is still being multiplied
         float zg[16], zu[16], yg[16], yu[16];
         if (KIND == FF_DGATE) ff_load_z(z, g.z_plane, 0 < z_cols, zg, zu);
-        const bool bad = !mbar_wait(acc_full + buf, (chunk >> 1) & 1) || *abort_flag != 0;
+        const bool bad = !ff_wait(acc_full + buf, (chunk >> 1) & 1, abort_flag) || *abort_flag != 0;
         if (ff_epi_bar_or<L::EPI>(bad)) stop = true;
         else {
           tc_fence_after();
@@ -670,13 +713,40 @@ __global__ void __launch_bounds__(FF_THREADS((FfnSmem<BN, S, KIND, CG>::EPI)), 1
           ++chunk;
         }
       }
-      if (stop) { *abort_flag = 1; break; }
+      if (stop) {
+        ff_give_up<CG>(abort_flag, rank);
+        break;
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync_all();    // the peer neither reads this CTA's shared memory nor signals its barriers any more
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ffn_error, 1);
+  if (*abort_flag) {      // the same in both CTAs of a pair
+    if (threadIdx.x == 0) atomicExch(&g_ffn_error, 1);
+    if (warp == L::EPI && rank == 0) {
+      // Copies: those of the last STAGES stages that either CTA has started.  One half of a pair's stage may not have been started;
+      // the leader then counts for it: its arrival where its own is missing, the bytes of the peer's half where that one is.
+      const uint32_t mine = *issued, peer = CG == 2 ? ff_peer_word(map_rank(const_cast<const uint32_t*>(issued), 1)) : mine;
+      const uint32_t end = mine > peer ? mine : peer;
+      for (uint32_t j = end > L::STAGES ? end - L::STAGES : 0; j < end; ++j) {
+        uint64_t* bar = full + j % L::STAGES;
+        if (CG == 2 && lane == 0) {
+          if (j >= mine) mbar_expect_tx(bar, L::STAGE);
+          if (j >= peer) ff_complete_tx(bar, L::STAGE);
+        }
+        __syncwarp();
+        mbar_wait(bar, (j / L::STAGES) & 1);
+      }
+    }
+    if (warp == L::EPI + 1) {
+      if (rank == 0 && elect_one()) ff_commit<CG>(drained);
+      __syncwarp();
+      mbar_wait(drained, 0);
+    }
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();
+  }
   if (warp == 0) {
     tc_fence_after();
     ff_tmem_free<CG>(tmem_base, TMEM_COLS);
@@ -823,6 +893,10 @@ struct FfnChain {
 };
 static thread_local FfnChain ffn_chain;      // of the call that this thread is in
 
+static std::atomic<int> ffn_give_up{0};
+// for tests: `give_up` of the launches that follow (FfnBatch); returns the one before
+extern "C" int gated_ffn_give_up(int how) { return ffn_give_up.exchange(how); }
+
 template <int BN, int S, int KIND, int CG>
 static int ffn_launch_t(FfnBatch& batch, const FfnOperands* o, cudaStream_t st) {
   void (*kernel)(FfnBatch) = ffn_gemm_kernel<BN, S, KIND, CG>;
@@ -845,6 +919,7 @@ static int ffn_launch_t(FfnBatch& batch, const FfnOperands* o, cudaStream_t st) 
     if (tiles > 0x3fffffffLL) return -1;
   }
   batch.first[batch.n] = (int)tiles;
+  batch.give_up = ffn_give_up;
   const int most = sm_count() / CG, grid = CG * (tiles < most ? (int)tiles : most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -1162,9 +1237,11 @@ extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
   return batch.n ? ffn_plain(S, plan, batch, index, o, dt, partial, st) : 0;
 }
 
-// 0, or 1 after a bounded wait of a kernel on the current device ran out (synchronises)
+// 0, or 1 after a bounded wait of a kernel on the current device ran out since the last call (synchronises)
 extern "C" int gated_ffn_last_error() {
   int v = -1;
-  cudaMemcpyFromSymbol(&v, g_ffn_error, sizeof(int));
+  if (cudaMemcpyFromSymbol(&v, g_ffn_error, sizeof(int)) != cudaSuccess) return -1;
+  const int none = 0;
+  if (v != 0) cudaMemcpyToSymbol(g_ffn_error, &none, sizeof(int));
   return v;
 }

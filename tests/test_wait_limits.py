@@ -1,4 +1,6 @@
 """What a kernel does when one of its bounded waits runs out: it leaves in order, waits for its copies in flight, and says so."""
+import random
+
 import pytest
 import torch
 
@@ -55,3 +57,99 @@ def test_layer_norm_ring_whose_waits_run_out(shape, dtype):
     for p, q in zip(torch.autograd.grad(want, (x, w, b), dy), grads):
         assert torch.equal(p, q)
     assert last_error() == 0
+
+
+# ---- gated feed-forward: what a pair of CTAs has in flight, restated ------------------------------------------------------
+class _Stage:
+    """An mbarrier with one arrival per phase and a byte count (in halves of a pair's stage)."""
+
+    def __init__(self):
+        self.phase, self.arrivals, self.tx = 0, 1, 0
+
+    def update(self, arrivals=0, tx=0):
+        self.arrivals -= arrivals
+        self.tx += tx
+        assert self.arrivals >= 0
+        if self.arrivals == 0 and self.tx == 0:
+            self.phase, self.arrivals = self.phase + 1, 1
+
+
+@pytest.mark.parametrize("ranks", [1, 2])
+@pytest.mark.parametrize("stages", [2, 3, 8])
+def test_gated_ffn_drains_what_both_ctas_have_in_flight(stages, ranks):
+    """Either CTA may stop at any stage.  The drain's waits all end, each only when the copies it stands for have landed, and nothing is
+    in flight behind it."""
+    rng = random.Random(stages)
+    for _ in range(400):
+        full = [_Stage() for _ in range(stages)]
+        stop = [rng.randrange(0, 3 * stages) for _ in range(ranks)]
+        issued, consumed, flying = [0] * ranks, 0, []
+
+        def land():
+            j = flying.pop(rng.randrange(len(flying)))
+            full[j % stages].update(tx=-1)
+
+        consume_to = rng.randrange(0, 3 * stages)
+        for _ in range(40 * stages):
+            r = rng.randrange(ranks + 2)
+            if r < ranks and issued[r] < stop[r] and issued[r] < consumed + stages:
+                j = issued[r]
+                if r == 0:
+                    full[j % stages].update(arrivals=1, tx=ranks)
+                flying.append(j)
+                issued[r] += 1
+            elif r == ranks and flying:
+                land()
+            elif r == ranks + 1 and consumed < consume_to and consumed < min(issued) and full[consumed % stages].phase > consumed // stages:
+                consumed += 1
+        mine, peer = issued[0], issued[-1]
+        end = max(mine, peer)
+        for j in range(max(0, end - stages), end):
+            bar, phase = full[j % stages], j // stages
+            assert bar.phase in (phase, phase + 1)           # a wait for the phase's parity means this phase
+            if ranks == 2:
+                if j >= mine:
+                    bar.update(arrivals=1, tx=1)
+                if j >= peer:
+                    bar.update(tx=-1)
+            while bar.phase == phase:
+                assert flying, "the wait would run out"
+                land()
+            assert j not in flying
+        assert not flying
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,d,f,n,dtype", [(2000, 1024, 2048, 1024, torch.bfloat16), (700, 520, 1304, 512, torch.float16),
+                                           (300, 200, 520, 200, torch.bfloat16), (33, 72, 136, 72, torch.bfloat16),
+                                           (1120, 650, 1300, 650, torch.float32), (70, 136, 200, 136, torch.float32)])
+def test_gated_ffn_whose_waits_run_out(m, d, f, n, dtype):
+    """One CTA of a pair, or both, give up some time into the kernel, with copies and multiplications in flight: the calls return, the error word
+    says so once, and the next calls are right."""
+    from chocosgd_b200.ops import _lib
+    from chocosgd_b200.ops.ffn import gated_ffn, last_error
+
+    lib = _lib.load()
+    torch.manual_seed(0)
+    leaves = [(torch.randn(*s, device="cuda") * s[1] ** -0.5).to(dtype).requires_grad_() for s in ((m, d), (2 * f, d), (n, f))]
+    dy = torch.randn(m, n, device="cuda").to(dtype)
+    y = gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    assert last_error() == 0
+    for ranks in (1, 2, 3):
+        for ns in (0, 500, 2000, 5000, 20000):
+            assert lib.gated_ffn_give_up(ns << 2 | ranks) == 0
+            try:
+                gated_ffn(*leaves)
+                late = last_error()
+                torch.autograd.grad(y, leaves, dy, retain_graph=True)
+                late_backward = last_error()
+            finally:
+                lib.gated_ffn_give_up(0)
+            if ranks != 2:                                  # rank 1 exists in launches of pairs only
+                assert late == 1 and late_backward == 1
+            assert last_error() == 0
+        assert torch.equal(gated_ffn(*leaves), y)
+        for p, q in zip(torch.autograd.grad(y, leaves, dy, retain_graph=True), grads):
+            assert torch.equal(p, q)
+        assert last_error() == 0
