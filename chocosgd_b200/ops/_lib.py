@@ -234,6 +234,18 @@ def ptr(t):
 _NODES = None
 
 
+def check_waits():
+    """Raise ``KernelTimeout`` if a bounded wait of a layer-norm or feed-forward kernel ran out on the current device since the last
+    call (synchronises).  Reads nothing in a process that has not used them."""
+    if _NODES is None:
+        return
+    late = [name for name in ("layer_norm", "gated_ffn") if getattr(load(), name + "_last_error")() != 0]
+    if late:
+        from ..utils.error_handler import KernelTimeout
+
+        raise KernelTimeout(late)
+
+
 def nodes():
     """The module of autograd nodes (``csrc/autograd.cpp``): layer_norm, dropout, gated_ffn."""
     global _NODES

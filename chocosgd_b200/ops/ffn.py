@@ -17,7 +17,8 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 
 
 def last_error() -> int:
-    """Non-zero after a bounded wait of one of the kernels on the current device ran out (synchronises)."""
+    """Non-zero if a bounded wait of one of the kernels on the current device ran out since the last call (synchronises); the
+    optimizers' ``check`` reads it in a training loop."""
     return _lib.load().gated_ffn_last_error()
 
 

@@ -12,7 +12,8 @@ from . import _lib
 
 
 def last_error() -> int:
-    """Non-zero after a bounded wait of one of the kernels on the current device ran out (synchronises)."""
+    """Non-zero if a bounded wait of one of the kernels on the current device ran out since the last call (synchronises); the
+    optimizers' ``check`` reads it in a training loop."""
     return _lib.load().layer_norm_last_error()
 
 

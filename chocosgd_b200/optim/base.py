@@ -189,12 +189,21 @@ class DistributedOptimizer(Optimizer):
 
     def check(self):
         """Raise ``GossipTimeout`` if a bounded device-side wait of any transport of this optimizer
-        ran out (synchronises the device)."""
+        ran out, ``KernelTimeout`` if one of the model's own kernels did (synchronises the device)."""
         if self.engine is not None:
             self.engine.check()
         for ex in (self._exchange, self._gather):
             if ex is not None and ex is not False and hasattr(ex, "check"):
                 ex.check()
+        self.check_kernels()
+
+    def check_kernels(self):
+        """Raise ``KernelTimeout`` if a bounded wait of the model's own kernels ran out (synchronises the device)."""
+        if self.device.type == "cuda":
+            from ..ops import _lib
+
+            with torch.cuda.device(self.device):
+                _lib.check_waits()
 
     # ---- hyper-parameters ------------------------------------------------------------
     @property

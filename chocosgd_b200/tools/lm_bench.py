@@ -79,7 +79,7 @@ def main(argv=None):
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
         ms = float(t)
     opt.finalize()
-    opt.engine.check()
+    opt.check()
     if rank == 0:
         print(json.dumps({"bench": "lstm_lm", "n_gpus": world, "tokens_per_s": B * T * world * a.steps / (ms * 1e-3),
                           "ms_per_step": ms / a.steps, "loss": float(loss), "graph": step.use_graph, "native": a.native, "ffn": a.ffn, "tf32_matmul": bool(a.tf32_matmul),

@@ -226,6 +226,7 @@ def do_validate(conf, graph, run, model, optimizer, criterion, scheduler, metric
     optimizer.finalize()
     performance = validate(conf, graph, run, model, optimizer, criterion, scheduler, metrics, data_loader,
                            device=device, rank_slice=rank_slice)
+    optimizer.check_kernels()       # before the result is taken for the best one, or saved
     perf0 = performance[0]
     scheduler.best_tracker.update(perf0, scheduler.epoch_)
     display_best_test_stat(run.logger, graph, scheduler)

@@ -25,6 +25,14 @@ class GossipTimeout(RuntimeError):
         self.status, self.peer, self.step = status, peer, step
 
 
+class KernelTimeout(RuntimeError):
+    """A bounded wait inside kernels of this process' own GPU ran out: their results are not to be used."""
+
+    def __init__(self, kernels):
+        super().__init__(f"a bounded wait ran out in {', '.join(kernels)}: results since the last check are not valid")
+        self.kernels = list(kernels)
+
+
 class PeerLost(RuntimeError):
     def __init__(self, ranks):
         super().__init__(f"lost peers: {sorted(ranks)}")

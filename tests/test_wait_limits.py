@@ -153,3 +153,113 @@ def test_gated_ffn_whose_waits_run_out(m, d, f, n, dtype):
         for p, q in zip(torch.autograd.grad(y, leaves, dy, retain_graph=True), grads):
             assert torch.equal(p, q)
         assert last_error() == 0
+
+
+# ---- the host's side ---------------------------------------------------------------------------------------------------------
+class _FakeLib:
+    def __init__(self, **words):
+        self.words, self.reads = words, 0
+
+    def __getattr__(self, name):
+        def read():
+            self.reads += 1
+            return self.words.pop(name, 0)                 # reading a word resets it
+
+        return read
+
+
+def test_error_words_end_in_an_exception(monkeypatch):
+    from chocosgd_b200.ops import _lib
+    from chocosgd_b200.utils.error_handler import KernelTimeout
+
+    for words, named in (({}, []), ({"layer_norm_last_error": 1}, ["layer_norm"]), ({"gated_ffn_last_error": -1}, ["gated_ffn"]),
+                         ({"layer_norm_last_error": 1, "gated_ffn_last_error": 1}, ["layer_norm", "gated_ffn"])):
+        lib = _FakeLib(**words)
+        monkeypatch.setattr(_lib, "load", lambda: lib)
+        monkeypatch.setattr(_lib, "_NODES", object())
+        if named:
+            with pytest.raises(KernelTimeout) as e:
+                _lib.check_waits()
+            assert e.value.kernels == named
+        _lib.check_waits()
+        monkeypatch.setattr(_lib, "_NODES", None)
+        reads = lib.reads
+        _lib.check_waits()                                 # none of the kernels has run in this process
+        assert lib.reads == reads
+
+
+def test_optimizers_read_the_error_words(monkeypatch):
+    import contextlib
+    import types
+
+    from chocosgd_b200.ops import _lib
+    from chocosgd_b200.optim.base import DistributedOptimizer
+    from chocosgd_b200.utils.error_handler import KernelTimeout
+
+    calls = []
+
+    def late():
+        calls.append(1)
+        raise KernelTimeout(["layer_norm"])
+
+    monkeypatch.setattr(_lib, "check_waits", late)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    for kind, n in (("cpu", 0), ("cuda", 1)):
+        stub = types.SimpleNamespace(engine=None, _exchange=None, _gather=False, device=torch.device(kind))
+        stub.check_kernels = lambda stub=stub: DistributedOptimizer.check_kernels(stub)
+        if n:
+            with pytest.raises(KernelTimeout):
+                DistributedOptimizer.check(stub)
+        else:
+            DistributedOptimizer.check(stub)
+        assert len(calls) == n
+
+
+def test_a_validation_is_not_used_before_the_error_words_are_read(monkeypatch):
+    import types
+
+    from chocosgd_b200.train import loops
+    from chocosgd_b200.utils.error_handler import KernelTimeout
+
+    def late():
+        raise KernelTimeout(["layer_norm"])
+
+    monkeypatch.setattr(loops, "validate", lambda *a, **k: [0.0])
+    optimizer = types.SimpleNamespace(finalize=lambda: None, check_kernels=late)
+    tracker = types.SimpleNamespace(best_tracker=None)       # not reached
+    with pytest.raises(KernelTimeout):
+        loops.do_validate(None, None, None, None, optimizer, None, tracker, None, None, None)
+
+
+@pytest.mark.gpu
+def test_a_training_step_with_a_late_kernel_is_reported():
+    from chocosgd_b200.config import get_args
+    from chocosgd_b200.models import define_model
+    from chocosgd_b200.ops import _lib
+    from chocosgd_b200.ops import nn as nnn
+    from chocosgd_b200.optim import define_optimizer
+    from chocosgd_b200.parallel.topology import Graph
+    from chocosgd_b200.utils.error_handler import KernelTimeout
+
+    conf = get_args(["--arch", "rnn_lm", "--optimizer", "parallel_choco_v", "--comm_op", "sign", "--graph_topology", "ring", "--lr", "0.5",
+                     "--drop_rate", "0.0", "--rnn_n_hidden", "64", "--rnn_n_ffn", "160", "--gossip_impl", "fused"])
+    graph = Graph("ring", 1, 0)
+    model = define_model(conf, graph, data_loader={"n_tokens": 300}, device=torch.device("cuda", 0), consistent=False, verbose=False)
+    opt = define_optimizer(conf, model, graph)
+    lib = _lib.load()
+    words = torch.randint(0, 300, (8, 40), device="cuda")
+    hidden = tuple(h.cuda() for h in model.init_hidden(40))
+    try:
+        nnn.set_native(True, which=("norm", "ffn"))
+        model(words, hidden)[0].sum().backward()
+        opt.check()
+        lib.gated_ffn_give_up(3)
+        model(words, hidden)[0].sum().backward()
+        lib.gated_ffn_give_up(0)
+        with pytest.raises(KernelTimeout, match="gated_ffn"):
+            opt.check()
+        opt.check()                                        # reported once
+        opt.finalize()
+    finally:
+        lib.gated_ffn_give_up(0)
+        nnn.set_native(False, which=("norm", "ffn"))
