@@ -100,7 +100,7 @@ Tensor layer_norm_run(const Tensor& x, const Tensor& x2, const Tensor& w, const 
   c.stream = stream_of(x);
   if (c.n > 0) {
     check(layer_norm_forward(&c), "layer_norm_forward");
-    ++g_launches;
+    g_launches += c.launches;
   }
   return y;
 }
@@ -150,7 +150,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     c.dt = dtype_code(x2.scalar_type()); c.w_dt = dtype_code(type);
     c.stream = stream_of(x2);
     check(layer_norm_backward(&c), "layer_norm_backward");
-    g_launches += partial.defined() ? 2 : 1;
+    g_launches += c.launches;
     return {dx, dw, db, Tensor()};
   }
 };
@@ -179,7 +179,7 @@ Tensor dropout_run(const Tensor& in, const Tensor& residual, const Tensor& key, 
   c.stream = stream_of(x);
   if (c.n > 0) {
     check(dropout_apply(&c), "dropout_apply");
-    ++g_launches;
+    g_launches += c.launches;
   }
   return y;
 }
@@ -291,7 +291,7 @@ Tensor ffn_run(const Tensor& x, const Tensor& x2, const Tensor& wi, const Tensor
   c.m = m; c.d = d; c.f = f; c.n = n; c.act = act; c.dt = dt; c.few = few;
   c.st = stream_of(x);
   check(gated_ffn_forward(&c), "gated_ffn_forward");
-  g_launches += 2 + (at.x >= 0 || at.w_in >= 0 || at.w_out >= 0) + (floats > 0);
+  g_launches += c.launches;
   *kept = buf;
   return y;
 }
@@ -353,7 +353,7 @@ struct GatedFfnFn : torch::autograd::Function<GatedFfnFn> {
     c.m = m; c.d = d; c.f = f; c.n = n; c.act = ctx->saved_data["act"].toInt(); c.dt = dt;
     c.st = stream_of(dy);
     check(gated_ffn_backward(&c), "gated_ffn_backward");
-    g_launches += 1 + (dx.defined() || dwi.defined()) + (dy_img >= 0 || c.make != 0) + (floats > 0);
+    g_launches += c.launches;
     return {dx, dwi, dwo, Tensor()};
   }
 };

@@ -123,8 +123,9 @@ static int dropout_launch(const void* x, const void* res, void* y, long long n, 
                               : launch_k(dropout_kernel<T, 1, false>, g, b, 0, st, px, pr, py, n, k, site, drop, scale));
 }
 
-extern "C" int dropout_apply(const DropoutCall* c) {
+extern "C" int dropout_apply(DropoutCall* c) {
   if (c->n <= 0 || c->drop < 0 || c->drop > 65535 || ((uintptr_t)c->key & 3) != 0) return -1;
+  c->launches = 1;
   const float scale = 65536.f / (65536.f - (float)c->drop);
   const uint32_t site = (uint32_t)c->site, drop = (uint32_t)c->drop;
   if (c->dt == DT_F32) return dropout_launch<float>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, (cudaStream_t)c->stream);

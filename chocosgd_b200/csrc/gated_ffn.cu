@@ -884,10 +884,10 @@ struct FfnOperands {
 // memory), unless they run for many tiles per SM (777 x 1111 x 2777 fp16, all launches of a training pass: 132 -> 127.6 us, 1120 x 650
 // x 2600 fp32 274 -> 270; 8192 x 2048 x 8192 bf16 2170 -> 2206 with them, so not there).
 struct FfnChain {
-  bool next = false;
+  int launches = 0;         // so far; every launch asks dependent() once
   bool dependent(bool few_tiles = true) {
-    const bool d = (next && few_tiles) || pdl_enabled();
-    next = true;
+    const bool d = (launches > 0 && few_tiles) || pdl_enabled();
+    ++launches;
     return d;
   }
 };
@@ -1134,7 +1134,7 @@ extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt
 // whether an evaluation pass takes the form for few tokens (`few` of gated_ffn_forward)
 extern "C" int gated_ffn_few(int m, int d, int f, int n, int dt) { return ffn_few_fits(m, d, f, n, dt); }
 
-extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
+static int ffn_forward(const FfnForwardCall* c) {
   const void *x = c->x, *w_in = c->w_in, *w_out = c->w_out;
   void *x_img = c->x_img, *in_img = c->in_img, *out_img = c->out_img, *h = c->h, *y = c->y;
   float *z = c->z, *partial = c->partial;
@@ -1142,9 +1142,12 @@ extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
   const int m = (int)c->m, d = (int)c->d, f = (int)c->f, n = (int)c->n, act = (int)c->act, dt = (int)c->dt;
   const cudaStream_t st = (cudaStream_t)c->st;
   const FfnShape s = {m, d, f, n, act, dt};
-  if (!ffn_shape_ok(s)) return -1;
   ffn_chain = FfnChain();
-  if (c->few) return ffn_few_forward(x, ldx, w_in, ld_in, w_out, ld_out, reinterpret_cast<float*>(h), y, m, d, f, n, act, dt, st);
+  if (!ffn_shape_ok(s)) return -1;
+  if (c->few) {
+    ffn_chain.launches = 2;
+    return ffn_few_forward(x, ldx, w_in, ld_in, w_out, ld_out, reinterpret_cast<float*>(h), y, m, d, f, n, act, dt, st);
+  }
   FfnOperand ox, oi, oo;
   FfnImages images = {};
   ffn_prepare(&ox, x, m, d, ldx, 1, dt, x_img, &images);
@@ -1175,7 +1178,7 @@ extern "C" int gated_ffn_forward(const FfnForwardCall* c) {
   return ffn_plain(S, ffn_plan(S, FF_PLAIN, &p, 1), batch, &index, &o, dt, partial, st);
 }
 
-extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
+static int ffn_backward(const FfnBackwardCall* c) {
   const void *x = c->x, *w_in = c->w_in, *w_out = c->w_out, *dy = c->dy, *h = c->h;
   void *x_img = c->x_img, *in_img = c->in_img, *out_img = c->out_img, *dy_img = c->dy_img, *dz = c->dz;
   void *dx = c->dx, *dw_in = c->dw_in, *dw_out = c->dw_out;
@@ -1184,8 +1187,8 @@ extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
   const int m = (int)c->m, d = (int)c->d, f = (int)c->f, n = (int)c->n, act = (int)c->act, dt = (int)c->dt;
   const cudaStream_t st = (cudaStream_t)c->st;
   const FfnShape s = {m, d, f, n, act, dt};
-  if (!ffn_shape_ok(s)) return -1;
   ffn_chain = FfnChain();
+  if (!ffn_shape_ok(s)) return -1;
   const int S = dt == DT_F32 ? 3 : 1;
   FfnOperand ox, oi, oo, oy;
   FfnImages images = {};
@@ -1235,6 +1238,17 @@ extern "C" int gated_ffn_backward(const FfnBackwardCall* c) {
     index[batch.n++] = 2;
   }
   return batch.n ? ffn_plain(S, plan, batch, index, o, dt, partial, st) : 0;
+}
+
+extern "C" int gated_ffn_forward(FfnForwardCall* c) {
+  const int rc = ffn_forward(c);
+  c->launches = ffn_chain.launches;
+  return rc;
+}
+extern "C" int gated_ffn_backward(FfnBackwardCall* c) {
+  const int rc = ffn_backward(c);
+  c->launches = ffn_chain.launches;
+  return rc;
 }
 
 // 0, or 1 after a bounded wait of a kernel on the current device ran out since the last call (synchronises)

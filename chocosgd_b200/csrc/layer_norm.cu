@@ -720,8 +720,12 @@ static int ln_fwd(const LnArgs& a, cudaStream_t st) {
   return ln_launch_fwd<T, V, 2>(a, st);
 }
 
+// what a call has done: partial rows (blocks of the backward kernel) and launches
+struct LnRun {
+  int blocks = 0, launches = 0;
+};
 template <typename T, int V, int E, bool RING>
-static int ln_launch_bwd(const LnArgs& a, int* blocks, cudaStream_t st) {
+static int ln_launch_bwd(const LnArgs& a, LnRun* run, cudaStream_t st) {
   const int threads = ln_threads(a.d, E);
   if (threads > 1024) return -1;
   const long long per_sm = (a.n + sm_count() - 1) / sm_count();
@@ -738,7 +742,7 @@ static int ln_launch_bwd(const LnArgs& a, int* blocks, cudaStream_t st) {
   }
   long long nb = (a.n + groups - 1) / groups;
   if (nb > sm_count()) nb = sm_count();
-  *blocks = (int)nb;
+  run->blocks = (int)nb;
   void (*kernel)(LnArgs, int, int) = nullptr;
   if constexpr (RING) kernel = ln_give_up ? ln_bwd_ring_kernel<T, E, true> : ln_bwd_ring_kernel<T, E, false>;
   else kernel = ln_bwd_kernel<T, V, E>;
@@ -750,7 +754,8 @@ static int ln_launch_bwd(const LnArgs& a, int* blocks, cudaStream_t st) {
 }
 
 template <typename T>
-static int ln_dispatch(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStream_t st) {
+static int ln_dispatch(const LnArgs& a, int dt, bool bwd, LnRun* run, cudaStream_t st) {
+  run->launches = 1;
   if (a.d > LN_MAX_ROW) {
     const long long nb = a.n < 2LL * sm_count() ? a.n : 2LL * sm_count();
     if (!bwd) return (int)launch_k(ln_fwd_long_kernel<T>, dim3((unsigned)nb), dim3(1024), 0, st, a);
@@ -758,10 +763,10 @@ static int ln_dispatch(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStrea
       int rc = (int)launch_k(ln_bwd_long_kernel<T>, dim3((unsigned)nb), dim3(1024), 0, st, a);
       if (rc) return rc;
     }
-    *blocks = 0;
+    run->launches = (a.dx != nullptr) + (a.partial != nullptr);
     if (a.partial == nullptr) return 0;
-    *blocks = (int)(a.n < 64 ? a.n : 64);
-    return (int)launch_k(ln_wgrad_long_kernel<T>, dim3((a.d + 255) / 256, *blocks), dim3(256), 0, st, a);
+    run->blocks = (int)(a.n < 64 ? a.n : 64);
+    return (int)launch_k(ln_wgrad_long_kernel<T>, dim3((a.d + 255) / 256, run->blocks), dim3(256), 0, st, a);
   }
   const int v = ln_vec(a, dt, bwd);
   constexpr int W = 16 / sizeof(T);
@@ -778,43 +783,46 @@ static int ln_dispatch(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStrea
   // 16: half the shuffles per element (16384 x 4096 bf16: 92 against 103 us, 65536 x 1024: 86 against 104).
   if (v == W) {
     if ((long long)a.d * (8 + LN_RING * 2 * (long long)sizeof(T)) <= 200 * 1024 && a.d <= 16 * LN_T16)
-      return a.d <= 8192 && (sizeof(T) == 4 || a.d < 1024) ? ln_launch_bwd<T, W, 8, true>(a, blocks, st)
-                                                            : ln_launch_bwd<T, W, 16, true>(a, blocks, st);
-    return a.d <= 8192 ? ln_launch_bwd<T, W, 8, false>(a, blocks, st) : ln_launch_bwd<T, W, 16, false>(a, blocks, st);
+      return a.d <= 8192 && (sizeof(T) == 4 || a.d < 1024) ? ln_launch_bwd<T, W, 8, true>(a, run, st)
+                                                            : ln_launch_bwd<T, W, 16, true>(a, run, st);
+    return a.d <= 8192 ? ln_launch_bwd<T, W, 8, false>(a, run, st) : ln_launch_bwd<T, W, 16, false>(a, run, st);
   }
-  if (v == 2) return a.d <= 8192 ? ln_launch_bwd<T, 2, 8, false>(a, blocks, st) : ln_launch_bwd<T, 2, 16, false>(a, blocks, st);
-  return a.d <= 8192 ? ln_launch_bwd<T, 1, 8, false>(a, blocks, st) : ln_launch_bwd<T, 1, 16, false>(a, blocks, st);
+  if (v == 2) return a.d <= 8192 ? ln_launch_bwd<T, 2, 8, false>(a, run, st) : ln_launch_bwd<T, 2, 16, false>(a, run, st);
+  return a.d <= 8192 ? ln_launch_bwd<T, 1, 8, false>(a, run, st) : ln_launch_bwd<T, 1, 16, false>(a, run, st);
 }
 
-static int ln_run(const LnArgs& a, int dt, bool bwd, int* blocks, cudaStream_t st) {
+static int ln_run(const LnArgs& a, int dt, bool bwd, LnRun* run, cudaStream_t st) {
   if (a.n <= 0 || a.d <= 0 || (a.ldx < a.d && a.n > 1 && a.ldx != 0) || a.w_dt < 0 || a.w_dt > 2) return -1;
-  if (dt == DT_F32) return ln_dispatch<float>(a, dt, bwd, blocks, st);
-  if (dt == DT_BF16) return ln_dispatch<__nv_bfloat16>(a, dt, bwd, blocks, st);
-  if (dt == DT_F16) return ln_dispatch<__half>(a, dt, bwd, blocks, st);
+  if (dt == DT_F32) return ln_dispatch<float>(a, dt, bwd, run, st);
+  if (dt == DT_BF16) return ln_dispatch<__nv_bfloat16>(a, dt, bwd, run, st);
+  if (dt == DT_F16) return ln_dispatch<__half>(a, dt, bwd, run, st);
   return -1;
 }
 
-extern "C" int layer_norm_forward(const LnForwardCall* c) {
+extern "C" int layer_norm_forward(LnForwardCall* c) {
   LnArgs a = {};
   a.x = c->x; a.w = c->w; a.b = c->b; a.y = c->y; a.n = c->n; a.ldx = c->ldx; a.d = (int)c->d; a.eps = (float)c->eps;
   a.w_dt = (int)c->w_dt;
   a.mean = c->stats;
   a.rstd = c->stats != nullptr ? c->stats + c->n : nullptr;
-  int blocks = 0;
-  return ln_run(a, (int)c->dt, false, &blocks, (cudaStream_t)c->stream);
+  LnRun run;
+  const int rc = ln_run(a, (int)c->dt, false, &run, (cudaStream_t)c->stream);
+  c->launches = run.launches;
+  return rc;
 }
 
-extern "C" int layer_norm_backward(const LnBackwardCall* c) {
+extern "C" int layer_norm_backward(LnBackwardCall* c) {
   if ((c->dw != nullptr || c->db != nullptr) != (c->partial != nullptr)) return -1;
   LnArgs a = {};
   a.x = c->x; a.dy = c->dy; a.lddy = c->lddy; a.w = c->w; a.mean = c->stats; a.rstd = c->stats + c->n;
   a.dx = c->dx; a.partial = c->partial; a.n = c->n; a.ldx = c->ldx; a.d = (int)c->d; a.w_dt = (int)c->w_dt;
-  int blocks = 0;
-  const int rc = ln_run(a, (int)c->dt, true, &blocks, (cudaStream_t)c->stream);
+  LnRun run;
+  const int rc = ln_run(a, (int)c->dt, true, &run, (cudaStream_t)c->stream);
+  c->launches = run.launches + (c->partial != nullptr);
   if (rc || c->partial == nullptr) return rc;
   // a programmatic dependent of the kernel before (1120 x 650 fp32, the whole training pass: 16.4 -> 15.7 us)
   return (int)launch_k_if(true, ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, (cudaStream_t)c->stream,
-                       (const float*)c->partial, blocks, a.d, c->dw, c->db, a.w_dt);
+                       (const float*)c->partial, run.blocks, a.d, c->dw, c->db, a.w_dt);
 }
 
 // 0, or 1 after a bounded wait of a kernel on the current device ran out since the last call (synchronises)
