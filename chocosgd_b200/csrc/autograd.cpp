@@ -206,7 +206,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
   }
 };
 
-// drop: the probability in steps of 2^-16, 0 .. 65535
+// drop: the probability in steps of 2^-16, 0 .. 65536
 Tensor dropout(const Tensor& x, int64_t drop, const Tensor& key, int64_t site, const Maybe& res) {
   const Tensor residual = res.value_or(Tensor());
   if (!x.is_cuda() || dtype_code(x.scalar_type()) < 0)

@@ -31,7 +31,7 @@ struct LnBackwardCall {
   long long launches;
 };
 
-// y[i] = res[i] + keep(i) x[i] 65536 / (65536 - drop), i < n; res may be null; key: 8 bytes on the device; drop = 0 .. 65535
+// y[i] = res[i] + keep(i) x[i] 65536 / (65536 - drop), i < n; res may be null; key: 8 bytes on the device; drop = 0 .. 65536 (nothing is kept)
 struct DropoutCall {
   const void *x, *res;
   void* y;

@@ -124,9 +124,9 @@ static int dropout_launch(const void* x, const void* res, void* y, long long n, 
 }
 
 extern "C" int dropout_apply(DropoutCall* c) {
-  if (c->n <= 0 || c->drop < 0 || c->drop > 65535 || ((uintptr_t)c->key & 3) != 0) return -1;
+  if (c->n <= 0 || c->drop < 0 || c->drop > 65536 || ((uintptr_t)c->key & 3) != 0) return -1;
   c->launches = 1;
-  const float scale = 65536.f / (65536.f - (float)c->drop);
+  const float scale = c->drop < 65536 ? 65536.f / (65536.f - (float)c->drop) : 0.f;      // 65536: no draw reaches it, nothing is kept
   const uint32_t site = (uint32_t)c->site, drop = (uint32_t)c->drop;
   if (c->dt == DT_F32) return dropout_launch<float>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, (cudaStream_t)c->stream);
   if (c->dt == DT_BF16) return dropout_launch<__nv_bfloat16>(c->x, c->res, c->y, c->n, c->key, site, drop, scale, (cudaStream_t)c->stream);

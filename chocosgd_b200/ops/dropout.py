@@ -36,9 +36,4 @@ def dropout(x, p: float, key, site: int = 0, residual=None):
         raise ValueError(f"dropout: the probability has to lie in [0, 1], got {p}")
     if not 0 <= site < 1 << 32:
         raise ValueError(f"dropout: site has to fit into 32 bits, got {site}")
-    drop = drop_steps(p)
-    if drop == 65536:                      # everything is dropped: as for p just below 1, with nothing left to scale
-        y = _lib.nodes().dropout(x, 65535, key, site, None)
-        y = torch.where(torch.zeros((), dtype=torch.bool, device=x.device), y, torch.zeros_like(y))
-        return y if residual is None else residual + y
-    return _lib.nodes().dropout(x, drop, key, site, residual)
+    return _lib.nodes().dropout(x, drop_steps(p), key, site, residual)

@@ -23,6 +23,7 @@ def test_entry_points_refuse_a_tangent_in_any_input():
     key = torch.tensor([3], device="cuda")
     calls = ((lambda *a: layer_norm(*a), layer_norm_supported, ((6, 8), (8,), (8,))),
              (lambda x, r: dropout(x, 0.5, key, residual=r), dropout_supported, ((6, 8), (6, 8))),
+             (lambda x, r: dropout(x, 1.0, key, residual=r), dropout_supported, ((6, 8), (6, 8))),
              (lambda *a: gated_ffn(*a), gated_ffn_supported, ((6, 8), (24, 8), (8, 12))))
     for call, supported, shapes in calls:
         for which in range(len(shapes)):
