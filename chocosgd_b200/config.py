@@ -255,7 +255,8 @@ def build_parser() -> argparse.ArgumentParser:
     )
     p.add_argument("--dtype", default="fp32", choices=("fp32", "bf16"))
     p.add_argument("--pdl", default="auto", choices=("auto", "on", "off"),
-                   help="programmatic dependent launch between the library's kernels (auto: on with --dtype bf16)")
+                   help="programmatic dependent launch between the library's kernels (auto: on with --dtype bf16, and in any case "
+                   "between the launches inside one call of layer norm or gated feed-forward; off: none)")
     p.add_argument("--steps", default=None, type=int, help="stop after this many local steps")
     p.add_argument("--wait_budget_ms", default=2000.0, type=float,
                    help="upper bound of every in-kernel wait on a peer flag")

@@ -886,7 +886,7 @@ struct FfnOperands {
 struct FfnChain {
   int launches = 0;         // so far; every launch asks dependent() once
   bool dependent(bool few_tiles = true) {
-    const bool d = (launches > 0 && few_tiles) || pdl_enabled();
+    const bool d = (launches > 0 && few_tiles && pdl_in_call()) || pdl_enabled();
     ++launches;
     return d;
   }
@@ -1239,6 +1239,9 @@ static int ffn_backward(const FfnBackwardCall* c) {
   }
   return batch.n ? ffn_plain(S, plan, batch, index, o, dt, partial, st) : 0;
 }
+
+// whether launches inside a call are programmatic dependents in this process
+extern "C" int choco_pdl_in_call() { return pdl_in_call() || pdl_enabled(); }
 
 extern "C" int gated_ffn_forward(FfnForwardCall* c) {
   const int rc = ffn_forward(c);

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(FEW_THREADS) ffn_few_kernel(FewArgs a) {
   }
 }
 
-// The second product is always launched as a programmatic dependent of the first (1 token, 2048 x 8192 bf16: 23.2 -> 21.9 us;
+// The second product is launched as a programmatic dependent of the first (1 token, 2048 x 8192 bf16: 23.2 -> 21.9 us;
 // with its weights prefetched into L2 before its wait 22.6).
 // Blocks: as many as fit on an SM by their registers (four, two), fewer for few columns.  Warps per row (k_split): the
 // cheapest by  rounds of a block x (steps x cycles of a step + cycles of bringing the sums together), with two to eight warps
@@ -170,7 +170,7 @@ static int few_launch(FewArgs& a, cudaStream_t st) {
     const long long cost = (long long)((groups + wr - 1) / wr) * ((long long)((steps + q - 1) / q) * step + join);
     if (cost < best) { best = cost; a.k_split = q; }
   }
-  return (int)launch_k_if(!GATE || pdl_enabled(), ffn_few_kernel<TW, TX, TO, MT, V, GATE>, dim3(grid), dim3(FEW_THREADS), 0, st, a);
+  return (int)launch_k_if((!GATE && pdl_in_call()) || pdl_enabled(), ffn_few_kernel<TW, TX, TO, MT, V, GATE>, dim3(grid), dim3(FEW_THREADS), 0, st, a);
 }
 // ---- more tokens: the warps' matrix instruction ------------------------------------------------------------------------
 // A block multiplies 32 tokens (8 NT) with 32 weight rows (gate: 16 gate rows and their up rows, which meet in one thread); its
@@ -379,7 +379,7 @@ static int fm_launch(FewArgs& a, cudaStream_t st) {
     at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (!GATE || pdl_enabled()) {
+  if ((!GATE && pdl_in_call()) || pdl_enabled()) {
     at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;

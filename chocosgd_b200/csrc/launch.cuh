@@ -11,8 +11,13 @@
 // Inside a captured CUDA graph the attribute becomes a programmatic dependency edge.  Without the
 // attribute (the default, or a launch by plain <<<>>>) both calls are no-ops.
 //
-// Switched by CHOCO_PDL (read at the first launch), which ops/_lib.py: configure_pdl() sets from --pdl: on for
-// bf16-autocast training, off otherwise.  Measured on B200: inside the captured fp32 ResNet-20 step (about 140
+// Two switches, read at the first launch; ops/_lib.py: configure_pdl() sets both from --pdl.
+//   CHOCO_PDL        between all kernels of the library: on for bf16-autocast training, off otherwise
+//   CHOCO_PDL_CALLS  between the launches of one call of an operator whose kernels follow each other closely (the layer-norm
+//                    backward pass and its reduction, the feed-forward products): on unless --pdl off, or CHOCO_PDL=0 by
+//                    itself, says otherwise.  1120 x 650 fp32 layer norm, training pass 16.4 -> 15.7 us; 777 x 1111 x 2777
+//                    fp16 feed-forward 132 -> 127; 1 token 2048 x 8192 bf16 23.2 -> 21.6.
+// CHOCO_PDL measured on B200: inside the captured fp32 ResNet-20 step (about 140
 // kernels of 3 - 10 us) programmatic edges made the step slower, 1.30 ms against 1.25 ms with plain edges (1.34 ms
 // when the trigger precedes the wait and several kernels of the chain become resident at once): a graph's
 // kernel-to-kernel hand-over is already cheaper than the bookkeeping of the early launch at that kernel size.
@@ -44,6 +49,17 @@ static inline bool pdl_enabled() {
   if (v < 0) {
     const char* e = getenv("CHOCO_PDL");
     v = (e != nullptr && atoi(e) != 0) ? 1 : 0;
+  }
+  return v != 0;
+}
+
+// whether a launch may be a programmatic dependent of the one before it in the same call
+static inline bool pdl_in_call() {
+  static int v = -1;
+  if (v < 0) {
+    const char* e = getenv("CHOCO_PDL_CALLS");
+    if (e == nullptr || *e == 0) e = getenv("CHOCO_PDL");
+    v = (e == nullptr || *e == 0 || atoi(e) != 0) ? 1 : 0;
   }
   return v != 0;
 }

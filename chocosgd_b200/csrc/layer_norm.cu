@@ -821,7 +821,7 @@ extern "C" int layer_norm_backward(LnBackwardCall* c) {
   c->launches = run.launches + (c->partial != nullptr);
   if (rc || c->partial == nullptr) return rc;
   // a programmatic dependent of the kernel before (1120 x 650 fp32, the whole training pass: 16.4 -> 15.7 us)
-  return (int)launch_k_if(true, ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, (cudaStream_t)c->stream,
+  return (int)launch_k_if(pdl_in_call() || pdl_enabled(), ln_reduce_kernel, dim3((unsigned)((2LL * a.d + 31) / 32)), dim3(1024), 0, (cudaStream_t)c->stream,
                        (const float*)c->partial, run.blocks, a.d, c->dw, c->db, a.w_dt);
 }
 

@@ -43,10 +43,14 @@ def configure_pdl(mode: str = "auto", bf16: bool = False) -> bool:
     """Programmatic dependent launch for the library's kernels (``csrc/launch.cuh`` reads ``CHOCO_PDL`` at the
     first launch, so call this before any).  ``auto``: on for bf16-autocast training (measured on the ResNet-50
     step: 12.45 - 12.65 ms against 12.76 - 12.78 ms), off otherwise (the fp32 ResNet-20 step, about 140 kernels
-    of 3 - 10 us, was slower with it).  A ``CHOCO_PDL`` already in the environment wins."""
+    of 3 - 10 us, was slower with it).  A ``CHOCO_PDL`` already in the environment wins.
+
+    ``CHOCO_PDL_CALLS`` is the same for the launches inside one call of layer norm or gated feed-forward, which
+    gain from it in either case: on, except that ``off`` (or a ``CHOCO_PDL=0`` in the environment) means none at all."""
     if "CHOCO_PDL" not in os.environ:
         on = mode == "on" or (mode == "auto" and bf16)
         os.environ["CHOCO_PDL"] = "1" if on else "0"
+        os.environ.setdefault("CHOCO_PDL_CALLS", "0" if mode == "off" else "1")
     return os.environ["CHOCO_PDL"] not in ("", "0")
 
 
