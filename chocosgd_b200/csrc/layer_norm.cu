@@ -4,7 +4,8 @@
 //   g = dy w;  dx = rs (g - mean(g) - z mean(g z));  dw = sum over rows of dy z;  db = sum over rows of dy
 //
 // Both directions are one pass over memory: a row is read once, kept on the SM (the variance is taken about the mean, not from
-// a sum of squares) and written once.  All statistics and sums are fp32.
+// a sum of squares, and z from x - mu, not from x rs - mu rs: 1 % of the time at 16384 x 4096 bf16) and written once.  All statistics
+// and sums are fp32.
 //
 // Forward: a row belongs to one warp (up to 64 bytes x 16 per lane as they lie in memory, no block barrier), to several for long
 // rows and where there are few rows; blocks walk over the rows with weight and bias in shared memory.
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(768, 1) ln_fwd_ring_kernel(LnArgs a, int threa
     s[0] = f2_sum(sum) + f2_sum(more);
     ln_group_sum<1>(s, red[group][1], group, t, threads);
     const float rs = 1.f / sqrtf(fmaf(s[0], inv_d, a.eps));
-    const F2 rs2 = f2(rs), off = f2(-mu * rs);
+    const F2 rs2 = f2(rs), off = f2(-mu);
     T* y = reinterpret_cast<T*>(a.y) + row * a.d;
 #pragma unroll
     for (int j = 0; j < NV; ++j) opaque(r[j].raw);
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(768, 1) ln_fwd_ring_kernel(LnArgs a, int threa
         ln_get2<V>(b_s, vectors, j * threads + t, b);
         F2 o[V / 2];
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) o[i] = f2_fma(f2_fma(pair_of(r[j], i), rs2, off), w[i], b[i]);
+        for (int i = 0; i < V / 2; ++i) o[i] = f2_fma((pair_of(r[j], i) + off) * rs2, w[i], b[i]);
         store_pairs(y + (j * threads + t) * V, o);
       }
     if (t == 0 && a.mean != nullptr) {
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(E == 8 ? 1024 : LN_T16, 1) ln_bwd_ring_kernel(
       break;
     }
     const uint4 *xs = reinterpret_cast<const uint4*>(mine + k * 2 * row_bytes), *gs = xs + vectors;
-    const F2 rs2 = f2(rs), off = f2(-mu * rs);
+    const F2 rs2 = f2(rs), off = f2(-mu);
     F2 s0 = f2(0.f), s1 = f2(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(E == 8 ? 1024 : LN_T16, 1) ln_bwd_ring_kernel(
         ln_get2<V>(w_s, vectors, v, w);
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
-          const F2 z = f2_fma(pair_of(px, i), rs2, off), g = pair_of(pg, i), gw = g * w[i];
+          const F2 z = (pair_of(px, i) + off) * rs2, g = pair_of(pg, i), gw = g * w[i];
           dw[j * V / 2 + i] = f2_fma(g, z, dw[j * V / 2 + i]);
           db[j * V / 2 + i] = db[j * V / 2 + i] + g;
           s0 = s0 + gw;
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(E == 8 ? 1024 : LN_T16, 1) ln_bwd_ring_kernel(
     if (threads == 32) __syncwarp();
     if (t == 0 && row + (LN_RING - 1) * stride < a.n) fill(row + (LN_RING - 1) * stride, (k + LN_RING - 1) % LN_RING);
     if (a.dx != nullptr) {
-      const F2 mg = f2(-s[0] * inv_d), mgz = f2(-s[1] * inv_d);
+      const F2 mg = f2(-s[0] * inv_d), mgz = f2(-s[1] * inv_d * rs);      // of x - mu
       T* dx = reinterpret_cast<T*>(a.dx) + row * a.d;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -436,10 +437,7 @@ __global__ void __launch_bounds__(E == 8 ? 1024 : LN_T16, 1) ln_bwd_ring_kernel(
           F2 w[V / 2], o[V / 2];
           ln_get2<V>(w_s, vectors, v, w);
 #pragma unroll
-          for (int i = 0; i < V / 2; ++i) {
-            const F2 z = f2_fma(pair_of(px, i), rs2, off);
-            o[i] = f2_fma(z, mgz, f2_fma(pair_of(pg, i), w[i], mg)) * rs2;
-          }
+          for (int i = 0; i < V / 2; ++i) o[i] = f2_fma(pair_of(px, i) + off, mgz, f2_fma(pair_of(pg, i), w[i], mg)) * rs2;
           store_pairs(dx + v * V, o);
         }
       }
