@@ -1131,6 +1131,27 @@ extern "C" long long gated_ffn_partial_floats(int m, int d, int f, int n, int dt
   return ffn_partial_floats(ffn_plan(S, FF_PLAIN, p, backward ? 3 : 1), p, backward ? 3 : 1);
 }
 
+// The tiles that a training pass runs with, for tests: launches gate, Y, dgate, gradients x (accumulator columns, CTAs per tile,
+// slices of k of up to three products)
+extern "C" void gated_ffn_plan(int m, int d, int f, int n, int dt, int* out) {
+  const int S = dt == DT_F32 ? 3 : 1;
+  FfnProduct p[3];
+  FfnPlan plan[4];
+  p[0] = ffn_product(S, m, 1, 2 * f, d, 1);
+  plan[0] = ffn_plan(S, FF_GATE, p, 1);
+  p[0] = ffn_y_product(S, m, f, n);
+  plan[1] = ffn_plan(S, FF_PLAIN, p, 1);
+  p[0] = ffn_product(S, m, 1, f, n, 1);
+  plan[2] = ffn_plan(S, FF_DGATE, p, 1);
+  ffn_grad_products(S, m, d, f, n, p);
+  plan[3] = ffn_plan(S, FF_PLAIN, p, 3);
+  for (int i = 0; i < 4; ++i) {
+    out[5 * i] = plan[i].bn;
+    out[5 * i + 1] = plan[i].cg;
+    for (int j = 0; j < 3; ++j) out[5 * i + 2 + j] = plan[i].splits[j];
+  }
+}
+
 // whether an evaluation pass takes the form for few tokens (`few` of gated_ffn_forward)
 extern "C" int gated_ffn_few(int m, int d, int f, int n, int dt) { return ffn_few_fits(m, d, f, n, dt); }
 
