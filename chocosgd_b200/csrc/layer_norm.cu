@@ -16,11 +16,15 @@
 // groups in shared memory and writes one partial row; a second kernel adds the partial rows in block order.  No atomics: the same
 // inputs give the same bits.
 //
-// Bound by memory: 16384 x 4096 bf16 forward 57 us (268 MB, 0.73 of the copy rate), backward 90 + 7 (403 MB, 0.64); 16384 x 2048
-// fp32 47 / 71 us (0.88).  Small ones by launch and latency: 1120 x 650 fp32 16 us for the three kernels.
+// Bound by memory for fp32: 16384 x 2048 forward 48 us (268 MB, 0.87 of the copy rate), backward with its reduction 67 (403 MB, 0.93).
+// 16-bit rows by the latency of a row's steps (load, sum, squares, scaling, with a barrier between them) at 24 warps per SM: 16384 x 4096
+// bf16 forward 53 us (0.78), backward 88 (0.71), with 54 % of the issue slots and half of the memory's cycles in use.  Small ones by
+// launch and latency: 1120 x 650 fp32 16 us for the three kernels.
 //
-// Rows that do not start on 16-byte boundaries take narrower accesses (V elements at a time; 65536 x 1027 fp16 17 and 25 % of the copy rate); rows too long for registers
-// (above 16384 elements) take the *_long kernels, which read the row again from L2.
+// Rows that do not start on 16-byte boundaries take narrower accesses (V elements at a time; 65536 x 1027 fp16 17 and 25 % of the copy
+// rate); of long rows, above 4096 elements forward (8192 where they are not off boundaries) and 8192 backward, a part of 0.1 to 0.9 KB per
+// thread spills to local memory; rows too long for registers (above 16384 elements) take the *_long kernels, which read the row again from L2, one element per access (4096 x 20000 bf16,
+// forward and backward 763 us, the library 418; 2048 x 20000 fp32 469 and 353).
 #include "block_calls.h"
 #include "launch.cuh"
 #include "tc_common.cuh"
@@ -178,9 +182,8 @@ __device__ __forceinline__ void ln_get2(const float* s, int vectors, int v, F2 (
 
 // Rows on 16-byte boundaries, four vectors per lane.  A group (one warp up to 1024 16-bit elements) has two rows or more of its
 // own coming into shared memory by bulk copies while it works on a third in registers; the stage is filled again as soon as
-// the registers have it.  Arithmetic in pairs of fp32 numbers: one element at a time the kernel is bound by issue (18 instructions
-// per element; 16384 x 4096 bf16: 85 us, with pairs and 8 vectors per lane 77, with 4 vectors 63,
-// with 768 threads 57; 65536 x 1024: 48).
+// the registers have it.  Arithmetic in pairs of fp32 numbers, which halves the instructions (16384 x 4096 bf16: one element at a time 85
+// us, with pairs and 8 vectors per lane 77, with 4 vectors 63, with 768 threads 57, with one vote per row on the wait 53; 65536 x 1024: 46).
 // GIVE_UP: the first wait counts as one that ran out (tests).
 template <typename T, int NV, bool GIVE_UP>
 __global__ void __launch_bounds__(768, 1) ln_fwd_ring_kernel(LnArgs a, int threads, int groups, int depth) {
