@@ -48,7 +48,7 @@ bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 void no_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), what, ": no forward-mode derivative (an input carries a tangent)");
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), what, ": no forward-mode derivative (an input or a gradient carries a tangent)");
 }
 void no_second_derivative(const char* what) {
   if (at::GradMode::is_enabled())
@@ -121,6 +121,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("layer_norm");
+    no_tangent("layer_norm", {&grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor dy2 = rows_of(grads[0]);
     const int64_t rows = ctx->saved_data["rows"].toInt(), width = dy2.size(1);
@@ -194,6 +195,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor key = ctx->get_saved_variables()[0], &dy = grads[0];
+    no_tangent("dropout", {&dy});
     static const int64_t one = 1;
     check_saved(key, key.numel() == 1 ? key.sizes() : at::IntArrayRef(one), at::kLong, dy.device(), "dropout");
     const int64_t drop = ctx->saved_data["drop"].toInt(), site = ctx->saved_data["site"].toInt();
@@ -310,6 +312,7 @@ struct GatedFfnFn : torch::autograd::Function<GatedFfnFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_second_derivative("gated_ffn");
+    no_tangent("gated_ffn", {&grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();

@@ -39,6 +39,24 @@ def test_entry_points_refuse_a_tangent_in_any_input():
 
 
 @pytest.mark.gpu
+def test_backward_passes_refuse_a_tangent_in_the_gradient():
+    """Forward over reverse where only what follows the operator is differentiated forwards."""
+    from chocosgd_b200.ops.dropout import dropout
+    from chocosgd_b200.ops.ffn import gated_ffn
+    from chocosgd_b200.ops.norm import layer_norm
+
+    key = torch.tensor([3], device="cuda")
+    w_in, w_out = torch.randn(24, 8, device="cuda"), torch.randn(8, 12, device="cuda")
+    for call in (layer_norm, lambda x: dropout(x, 0.5, key), lambda x: gated_ffn(x, w_in, w_out)):
+        x = torch.randn(6, 8, device="cuda", requires_grad=True)
+        with fwAD.dual_level():
+            scale = fwAD.make_dual(torch.randn(6, 8, device="cuda"), torch.randn(6, 8, device="cuda"))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad((call(x) * scale).sum(), x)
+            torch.autograd.grad(call(x).sum(), x)
+
+
+@pytest.mark.gpu
 def test_layers_carry_the_tangent():
     from chocosgd_b200.models import layers as L
     from chocosgd_b200.ops import nn as nnn
