@@ -6,8 +6,11 @@ Here a run can continue on the survivors:
 
 * ``Heartbeat`` - every rank publishes its step in the rendezvous key-value store between steps
   (never while a kernel or collective of its own is in flight) and reads the others' keys; a rank
-  that leaves writes ``-1`` first, a rank that died is noticed when its key stops advancing for
+  that leaves before step ``s`` writes ``-s`` first, a rank that died is noticed when its key stops advancing for
   ``stale_after_s`` seconds;
+* where exchanges block the host, a rank enters a step only when every other one has entered it or has left before
+  it (``Membership.wait_entered``): all of them notice an announced exit at the same step, none waits for an
+  exchange that its neighbours will not post;
 * on the device every wait on a peer flag is bounded and ends in a status word
   (``utils.error_handler.GossipTimeout``), so a vanished peer can never hang a GPU; the trainer
   turns such a timeout into a membership check;
@@ -43,11 +46,12 @@ class Heartbeat:
     def beat(self, step: int):
         self.store.set(self._key(self.rank), str(int(step)))
 
-    def leave(self):
-        """Announce an orderly exit (call between steps)."""
-        self.store.set(self._key(self.rank), "-1")
+    def leave(self, step: int = 1):
+        """Announce an orderly exit (call between steps): this rank takes part in the steps before ``step``."""
+        self.store.set(self._key(self.rank), str(-int(step)))
 
-    def lost_peers(self) -> List[int]:
+    def lost_peers(self, step: Optional[int] = None) -> List[int]:
+        """Ranks that left (before ``step``, where one is given) or went silent."""
         now, lost = time.time(), []
         for r in self.peers:
             try:
@@ -55,7 +59,8 @@ class Heartbeat:
             except Exception:
                 continue
             if v < 0:
-                lost.append(r)
+                if step is None or -v <= step:
+                    lost.append(r)
                 continue
             last = self._seen.get(r)
             if last is None or last[0] != v:
@@ -63,6 +68,18 @@ class Heartbeat:
             elif self.stale_after_s is not None and now - last[1] > self.stale_after_s:
                 lost.append(r)
         return lost
+
+    def behind(self, step: int) -> List[int]:
+        """Ranks that have neither entered ``step`` nor announced that they leave."""
+        late = []
+        for r in self.peers:
+            try:
+                v = int(self.store.get(self._key(r)).decode())
+            except Exception:
+                continue
+            if 0 <= v < step:
+                late.append(r)
+        return late
 
     def check(self, step: int):
         """Publish this rank's step, raise ``PeerLost`` if a watched rank left or went silent."""
@@ -98,11 +115,22 @@ class Membership:
     def beat(self, step):
         self.heartbeat.beat(step)
 
-    def leave(self):
-        self.heartbeat.leave()
+    def leave(self, step: int = 1):
+        self.heartbeat.leave(step)
 
-    def lost(self) -> List[int]:
-        return self.heartbeat.lost_peers()
+    def lost(self, step: Optional[int] = None) -> List[int]:
+        return self.heartbeat.lost_peers(step)
+
+    def wait_entered(self, step: int, timeout_s: float = 30.0) -> List[int]:
+        """Wait until every member has entered ``step`` (``beat``) or one of them has left before it -> the ranks lost.  After
+        ``timeout_s`` the wait ends as if all had come (a slow rank; a dead one is noticed as without this call)."""
+        deadline = time.time() + timeout_s
+        while True:
+            late = self.heartbeat.behind(step)       # before the losses: who is not behind has left or entered by then
+            lost = self.lost(step)
+            if lost or not late or time.time() > deadline:
+                return lost
+            time.sleep(0.002)
 
     def agree(self, seen_lost: Sequence[int], step: int = 0, timeout_s: float = 30.0):
         """-> ``(lost, resume_step)``: the union of what every survivor saw, and the largest step index

@@ -52,11 +52,11 @@ class _Elastic:
     def wants_to_leave(self, global_rank, step) -> bool:
         return self.leave_rank == global_rank and step >= self.leave_step
 
-    def leave(self, optimizer):
+    def leave(self, optimizer, step):
         optimizer.finalize()
         if torch.cuda.is_available():
             torch.cuda.synchronize()
-        self.m.leave()
+        self.m.leave(step)
 
     def lost_now(self, optimizer, step, force=False):
         """-> global ranks lost, or [] (cheap: one store write; reads only at check points)."""
@@ -69,7 +69,9 @@ class _Elastic:
                 optimizer.check()
             except GossipTimeout as e:
                 timed_out = e
-            lost = self.m.lost()
+            # an exchange on the host blocks until the neighbours post theirs: nobody enters the step ahead of a rank that
+            # will see a loss there (the fused engine's waits are bounded on the device instead)
+            lost = self.m.wait_entered(step) if getattr(optimizer, "engine", None) is None else self.m.lost(step)
             if timed_out is not None and not lost:
                 # a peer stopped publishing payloads: give its heartbeat the chance to go stale
                 deadline = time.time() + (self.m.stale_after_s or 5.0) + 1.0
@@ -267,7 +269,7 @@ def train_and_validate(conf, graph, run, model, criterion, scheduler, optimizer,
         for _input, _target in data_loader["train_loader"]:
             if elastic is not None:
                 if elastic.wants_to_leave(global_rank, scheduler.local_index + 1):
-                    elastic.leave(optimizer)
+                    elastic.leave(optimizer, scheduler.local_index + 1)
                     logger.save_json()
                     run.extras["lost_ranks"] = [global_rank]
                     return scheduler

@@ -162,3 +162,33 @@ def test_training_continues_on_the_survivors(tmp_path):
     assert "lost ranks [2]: continuing on 3 nodes" in open(root / "0" / "log.txt").read()
     left = json.load(open(root / "2" / "log-1.json"))
     assert max(x["local_index"] for x in left if x.get("split") == "train") == 2
+
+
+def test_an_announced_exit_is_noticed_at_its_step():
+    """A rank that leaves before step 3 still counts in steps 1 and 2; a rank enters a step when the others have, or one has left."""
+    import threading
+
+    from chocosgd_b200.parallel.elastic import Membership
+
+    class Store(_FakeStore):
+        def check(self, keys):
+            return all(k in self.d for k in keys)
+
+    store = Store()
+    a, b, c = (Membership(store, r, [0, 1, 2]) for r in range(3))
+    for m in (a, b, c):
+        m.beat(1)
+    assert a.wait_entered(1, timeout_s=5) == []
+    a.beat(2)
+    t0 = time.time()
+    assert a.wait_entered(2, timeout_s=0.2) == [] and time.time() - t0 >= 0.2      # nobody else is there, nobody has left
+    b.beat(2)
+    threading.Timer(0.1, lambda: c.leave(3)).start()                               # c has entered step 2 by now, and leaves before 3
+    t0 = time.time()
+    assert a.wait_entered(2, timeout_s=5) == [] and time.time() - t0 < 4
+    assert a.lost(2) == [] and a.lost(3) == [2] and a.lost() == [2]
+    a.beat(3)
+    b.beat(3)
+    assert a.wait_entered(3, timeout_s=5) == [2] and b.wait_entered(3, timeout_s=5) == [2]
+    b.leave()                                                                      # without a step: at once
+    assert a.lost(1) == [1] and sorted(a.lost()) == [1, 2]
